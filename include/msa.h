@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MSA_ABI_VERSION 15
+#define MSA_ABI_VERSION 16
 
 /* status codes (negative: validation, nothing launched) */
 #define MSA_OK 0
@@ -352,6 +352,42 @@ int msa_decode_attention(const msa_tensor4* q, const msa_tensor4* k, const msa_t
 int msa_decode_attention_noalloc(const msa_tensor4* q, const msa_tensor4* k,
                                  const msa_tensor4* v, const msa_tensor4* o, float scale,
                                  msa_stream_t stream);
+
+/* Attention of a batch whose sequences share a prefix (no counterpart in the
+ * reference, whose decode takes one cache per sequence,
+ * minference/backend_npu/attention.py:274-314).  Row (b, h, i) sees every key
+ * of the prefix and keys j <= n_b - S_q + i of its sequence's own cache, n_b =
+ * lens[b] clamped to [0, S_c]: the S_q query rows are the last of the sequence.
+ *   q [B][H][S_q][D]; kp, vp [1][H_kv][S_p][D]; k, v [B][H_kv][S_c][D]
+ *   lens [B] int32 (device), or NULL: S_c for every sequence
+ * Any strides with D contiguous and 16-byte rows; S_p = 0 or S_c = 0 leaves
+ * that part out (its data pointers are not read).  o may be q's dtype or fp32.
+ * Own keys at and behind n_b are not used, whatever they hold.  Rows that see no key
+ * (or only scores of -inf) are written as 0.  Two launches: partial results of
+ * (rows, key range) items, and their merge. */
+size_t msa_shared_prefix_workspace_bytes(const msa_tensor4* q, const msa_tensor4* kp,
+                                         const msa_tensor4* vp, const msa_tensor4* k,
+                                         const msa_tensor4* v);
+int msa_shared_prefix_attention(const msa_tensor4* q, const msa_tensor4* kp, const msa_tensor4* vp,
+                                const msa_tensor4* k, const msa_tensor4* v, const msa_tensor4* o,
+                                const int32_t* lens, float scale, void* workspace,
+                                size_t workspace_bytes, msa_stream_t stream);
+
+/* msa_decode_attention over the first n_b = lens[b] (clamped to [0, S_k])
+ * keys of each sequence's cache, which also adds the attention weights to a
+ * score per key (no counterpart in the reference, which keeps every key):
+ *   scores_out[b][g][j] = scores_in[b][g][j] + sum over the heads h of kv head
+ *                         g of softmax(q_bh . k_bg * scale)[j],   j < n_b
+ * scores_out may be scores_in; entries from n_b on are left as they are.
+ *   q [B][H][1][D]; k, v [B][H_kv][S_k][D]; lens as above
+ *   scores_in, scores_out: fp32 described as [B][H_kv][S_k][1], stride[2] = 1
+ * Sums in a fixed order: the same call gives the same bits. */
+size_t msa_decode_accumulate_workspace_bytes(const msa_tensor4* q, const msa_tensor4* k,
+                                             const msa_tensor4* v);
+int msa_decode_accumulate(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* v,
+                          const msa_tensor4* o, const int32_t* lens, const msa_tensor4* scores_in,
+                          const msa_tensor4* scores_out, float scale, void* workspace,
+                          size_t workspace_bytes, msa_stream_t stream);
 
 /* Rotary position embedding of one layer's query and key heads, one launch.
  * Replaces the apply_rotary_pos_emb call of the patched forward

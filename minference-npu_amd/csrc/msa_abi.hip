@@ -1273,6 +1273,216 @@ int msa_decode_attention_noalloc(const msa_tensor4* q, const msa_tensor4* k,
   return msa_decode_attention(q, k, v, o, scale, ws, MSA_DECODE_SCRATCH_BYTES, stream);
 }
 
+// ---------------------------------------------------------------------------
+// rows against a shared prefix and their own caches; decode with the weights
+// ---------------------------------------------------------------------------
+namespace {
+
+// Keys of one item's range at most: its buffer descriptors cover below 2 GiB.
+int64_t rows_max_chunk(const msa_tensor4* k, const msa_tensor4* v) {
+  const int64_t row = std::max({k->stride[2], v->stride[2], k->size[3]}) * 2;
+  return ((int64_t(1) << 31) - 1024) / row / 128 * 128;
+}
+
+// `n` keys cut into about `want` ranges of whole 128-key rounds of the four
+// waves.
+void rows_split(int64_t n, int64_t want, int64_t max_chunk, int& n_split, int& chunk) {
+  if (n == 0) {
+    n_split = 0;
+    chunk = 128;
+    return;
+  }
+  const int64_t c = cdiv(cdiv(n, std::max<int64_t>(1, want)), 128) * 128;
+  chunk = int(std::min(c, max_chunk));
+  n_split = int(cdiv(n, chunk));
+}
+
+// Items of a call: the row tiles and key splits of the prefix (kp, or null)
+// and of the own caches.
+int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const msa_tensor4* vp,
+              const msa_tensor4* k, const msa_tensor4* v) {
+  const int64_t B = q->size[0], H = q->size[1], Sq = q->size[2], D = q->size[3];
+  const int64_t Hkv = k->size[1], G = H / Hkv;
+  const int64_t Sp = kp ? kp->size[2] : 0, Sc = k->size[2];
+  const int64_t rows = G * Sq, R = B * rows;
+  if (B > (1 << 24) || H > (1 << 24) || B * H > (1 << 24) || B * H * Sq > (1 << 24))
+    return MSA_E_HEADS;
+  rp.batch = int(B);
+  rp.heads = int(H);
+  rp.kv_heads = int(Hkv);
+  rp.group = int(G);
+  rp.s_q = int(Sq);
+  rp.s_p = int(Sp);
+  rp.s_c = int(Sc);
+  rp.mt = D > 128 || R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  rp.n_rt = int(cdiv(R, 16 * rp.mt));
+  rp.n_rto = int(cdiv(rows, 16));
+  const int64_t slots = 512;
+  rows_split(Sp, std::min<int64_t>(cdiv(Sp, 256), cdiv(slots, rp.n_rt * Hkv)),
+             kp ? rows_max_chunk(kp, vp) : 128, rp.n_sp, rp.chunk_p);
+  rows_split(Sc, std::min<int64_t>(cdiv(Sc, 256), cdiv(slots, rp.n_rto * B * Hkv)),
+             rows_max_chunk(k, v), rp.n_so, rp.chunk_o);
+  if (rp.n_sp + rp.n_so > kRowsMaxSplit) return MSA_E_SEQ;
+  const int64_t np = Hkv * rp.n_sp * rp.n_rt, no = B * Hkv * rp.n_so * rp.n_rto;
+  if (np + no >= (int64_t(1) << 31)) return MSA_E_HEADS;
+  rp.n_prefix_items = int(np);
+  rp.n_items = int(np + no);
+  rp.own_row0 = Hkv * rp.n_sp * R;
+  return MSA_OK;
+}
+
+// Workspace: part, then ml, then (decode_accumulate) the raw scores.
+struct RowsLayout {
+  size_t ml, raw, total;
+};
+RowsLayout rows_layout(const RowsParams& rp, int64_t D, bool raw) {
+  const size_t n = size_t(rp.own_row0 + int64_t(rp.batch) * rp.heads * rp.s_q * rp.n_so);
+  const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  RowsLayout l;
+  l.ml = up(n * size_t(D) * 4);
+  l.raw = l.ml + up(n * 8);
+  l.total = l.raw + (raw ? up(size_t(rp.batch) * rp.heads * rp.s_c * 4) : 0);
+  if (l.total == 0) l.total = 256;
+  return l;
+}
+
+// A cache pair of the rows kernels against q: sizes [batch][kv heads][any][D].
+int check_cache(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* v, int64_t batch) {
+  for (int i = 0; i < 4; ++i)
+    if (k->size[i] != v->size[i]) return MSA_E_RANK;
+  if (k->size[0] != batch || k->size[1] <= 0 || k->size[2] < 0 || k->size[3] != q->size[3])
+    return MSA_E_RANK;
+  if (k->dtype != q->dtype || v->dtype != q->dtype) return MSA_E_DTYPE;
+  if (k->size[2] == 0) return MSA_OK;
+  if (!k->data || !v->data) return MSA_E_NULL;
+  if (!aligned(k) || !aligned(v)) return MSA_E_ALIGN;
+  if (k->size[2] > kMaxSeq || rows_max_chunk(k, v) < 128) return MSA_E_SEQ;
+  return MSA_OK;
+}
+
+// q and o of the rows kernels.
+int check_rows_qo(const msa_tensor4* q, const msa_tensor4* o, float scale) {
+  if (!q->data || !o->data) return MSA_E_NULL;
+  for (int i = 0; i < 4; ++i)
+    if (q->size[i] <= 0 || o->size[i] != q->size[i]) return MSA_E_RANK;
+  if (q->dtype != MSA_DTYPE_BF16 && q->dtype != MSA_DTYPE_FP16) return MSA_E_DTYPE;
+  if (o->dtype != q->dtype && o->dtype != MSA_DTYPE_FP32) return MSA_E_DTYPE;
+  if (!head_dim_ok(q->size[3])) return MSA_E_HEAD_DIM;
+  if (!aligned(q) || !aligned(o)) return MSA_E_ALIGN;
+  if (q->size[2] > kMaxSeq) return MSA_E_SEQ;
+  if (!(scale > 0.0f) || !isfinite(scale)) return MSA_E_HEADS;
+  return MSA_OK;
+}
+
+void rows_fill(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* v,
+               const msa_tensor4* o, const int32_t* lens, float scale, const RowsLayout& l,
+               void* workspace) {
+  rp.q = q->data; rp.k = k->data; rp.v = v->data; rp.o = o->data;
+  rp.q_sb = q->stride[0]; rp.q_sh = q->stride[1]; rp.q_ss = q->stride[2];
+  rp.k_sb = k->stride[0]; rp.k_sh = k->stride[1]; rp.k_ss = k->stride[2];
+  rp.v_sb = v->stride[0]; rp.v_sh = v->stride[1]; rp.v_ss = v->stride[2];
+  rp.o_sb = o->stride[0]; rp.o_sh = o->stride[1]; rp.o_ss = o->stride[2];
+  rp.lens = lens;
+  rp.scale_log2 = float(double(scale) * 1.4426950408889634);
+  rp.part = ws_at<float>(workspace, 0);
+  rp.ml = ws_at<float>(workspace, l.ml);
+  rp.raw = ws_at<float>(workspace, l.raw);
+}
+
+bool rows_sizes_ok(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* v) {
+  for (int i = 0; i < 4; ++i)
+    if (q->size[i] <= 0) return false;
+  return q->size[2] <= kMaxSeq && k->size[1] > 0 && q->size[1] % k->size[1] == 0 &&
+         k->size[2] >= 0 && k->size[2] <= kMaxSeq &&
+         (k->size[2] == 0 || (k->size[3] > 0 && rows_max_chunk(k, v) >= 128));
+}
+
+}  // namespace
+
+size_t msa_shared_prefix_workspace_bytes(const msa_tensor4* q, const msa_tensor4* kp,
+                                         const msa_tensor4* vp, const msa_tensor4* k,
+                                         const msa_tensor4* v) {
+  if (!q || !kp || !vp || !k || !v || !rows_sizes_ok(q, k, v) || !rows_sizes_ok(q, kp, vp)) return 0;
+  RowsParams rp;
+  memset(&rp, 0, sizeof(rp));
+  if (rows_plan(rp, q, kp, vp, k, v) != MSA_OK) return 0;
+  return rows_layout(rp, q->size[3], false).total;
+}
+
+int msa_shared_prefix_attention(const msa_tensor4* q, const msa_tensor4* kp, const msa_tensor4* vp,
+                                const msa_tensor4* k, const msa_tensor4* v, const msa_tensor4* o,
+                                const int32_t* lens, float scale, void* workspace,
+                                size_t workspace_bytes, msa_stream_t stream) {
+  if (!q || !kp || !vp || !k || !v || !o) return MSA_E_NULL;
+  int st = check_rows_qo(q, o, scale);
+  if (st == MSA_OK) st = check_cache(q, kp, vp, 1);
+  if (st == MSA_OK) st = check_cache(q, k, v, q->size[0]);
+  if (st != MSA_OK) return st;
+  if (k->size[1] != kp->size[1] || q->size[1] % k->size[1] != 0) return MSA_E_RANK;
+  RowsParams rp;
+  memset(&rp, 0, sizeof(rp));
+  st = rows_plan(rp, q, kp, vp, k, v);
+  if (st != MSA_OK) return st;
+  const RowsLayout l = rows_layout(rp, q->size[3], false);
+  if (!workspace || workspace_bytes < l.total) return MSA_E_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return MSA_E_ALIGN;
+  rows_fill(rp, q, k, v, o, lens, scale, l, workspace);
+  rp.kp = kp->data; rp.vp = vp->data;
+  rp.kp_sh = kp->stride[1]; rp.kp_ss = kp->stride[2];
+  rp.vp_sh = vp->stride[1]; rp.vp_ss = vp->stride[2];
+  const hipError_t e = launch_rows(rp, false, q->dtype, o->dtype, int(q->size[3]),
+                                   reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSA_OK : int(e);
+}
+
+size_t msa_decode_accumulate_workspace_bytes(const msa_tensor4* q, const msa_tensor4* k,
+                                             const msa_tensor4* v) {
+  if (!q || !k || !v || !rows_sizes_ok(q, k, v)) return 0;
+  RowsParams rp;
+  memset(&rp, 0, sizeof(rp));
+  if (rows_plan(rp, q, nullptr, nullptr, k, v) != MSA_OK) return 0;
+  return rows_layout(rp, q->size[3], true).total;
+}
+
+int msa_decode_accumulate(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* v,
+                          const msa_tensor4* o, const int32_t* lens, const msa_tensor4* scores_in,
+                          const msa_tensor4* scores_out, float scale, void* workspace,
+                          size_t workspace_bytes, msa_stream_t stream) {
+  if (!q || !k || !v || !o || !scores_in || !scores_out) return MSA_E_NULL;
+  int st = check_rows_qo(q, o, scale);
+  if (st == MSA_OK) st = check_cache(q, k, v, q->size[0]);
+  if (st != MSA_OK) return st;
+  if (q->size[1] % k->size[1] != 0) return MSA_E_RANK;
+  if (q->size[2] != 1) return MSA_E_SEQ;
+  if (q->size[1] / k->size[1] > MSA_MAX_HEADS) return MSA_E_HEADS;
+  for (const msa_tensor4* s : {scores_in, scores_out}) {
+    if (s->size[0] != k->size[0] || s->size[1] != k->size[1] || s->size[2] != k->size[2] ||
+        s->size[3] != 1)
+      return MSA_E_RANK;
+    if (s->dtype != MSA_DTYPE_FP32) return MSA_E_DTYPE;
+    if (s->size[2] == 0) continue;
+    if (!s->data) return MSA_E_NULL;
+    if ((s->size[2] > 1 && s->stride[2] != 1) || (reinterpret_cast<uintptr_t>(s->data) & 3u) != 0)
+      return MSA_E_ALIGN;
+  }
+  if (q->size[0] * k->size[1] > 65535) return MSA_E_HEADS;
+  RowsParams rp;
+  memset(&rp, 0, sizeof(rp));
+  st = rows_plan(rp, q, nullptr, nullptr, k, v);
+  if (st != MSA_OK) return st;
+  const RowsLayout l = rows_layout(rp, q->size[3], true);
+  if (!workspace || workspace_bytes < l.total) return MSA_E_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return MSA_E_ALIGN;
+  rows_fill(rp, q, k, v, o, lens, scale, l, workspace);
+  rp.w_in = static_cast<const float*>(scores_in->data);
+  rp.w_out = static_cast<float*>(scores_out->data);
+  rp.wi_sb = scores_in->stride[0]; rp.wi_sh = scores_in->stride[1];
+  rp.wo_sb = scores_out->stride[0]; rp.wo_sh = scores_out->stride[1];
+  const hipError_t e = launch_rows(rp, true, q->dtype, o->dtype, int(q->size[3]),
+                                   reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSA_OK : int(e);
+}
+
 int msa_rope_qk(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* cos,
                 const msa_tensor4* sin, const msa_tensor4* q_out, const msa_tensor4* k_out,
                 msa_stream_t stream) {

@@ -220,6 +220,39 @@ struct DecodeParams {
   float* ml;           // workspace [batch*heads][n_split][2]: (m, l) per split
 };
 
+// Rows against a shared prefix and their own caches, or decode with the
+// attention weights (rows_kernel and the launch that merges its items).
+// Row r of kv head kvh: sequence r / (group * s_q), head kvh * group + r / s_q
+// % group, position r % s_q.
+struct RowsParams {
+  const void* q;   // [batch][heads][s_q][D]
+  const void* kp;  // prefix [kv_heads][s_p][D]
+  const void* vp;
+  const void* k;   // own caches [batch][kv_heads][s_c][D]
+  const void* v;
+  void* o;
+  int64_t q_sb, q_sh, q_ss;
+  int64_t kp_sh, kp_ss, vp_sh, vp_ss;
+  int64_t k_sb, k_sh, k_ss, v_sb, v_sh, v_ss;
+  int64_t o_sb, o_sh, o_ss;
+  const int32_t* lens;  // [batch] keys of each own cache, or nullptr: s_c
+  int batch, heads, kv_heads, group, s_q, s_p, s_c;
+  int mt;                    // 16-row tiles of a prefix item
+  int n_rt, n_sp, chunk_p;   // prefix: row tiles, key splits, keys of a split
+  int n_rto, n_so, chunk_o;  // own caches: the same per (sequence, kv head)
+  int n_prefix_items, n_items;
+  float scale_log2;          // softmax scale * log2(e)
+  float* part;               // partial O, [row][D]: prefix [kv_heads][n_sp][batch * rows],
+                             // from own_row0 on own [batch][kv_heads][n_so][rows]
+  float* ml;                 // (m, l) of each row of part
+  int64_t own_row0;
+  float* raw;                // decode_accumulate: raw scores [batch][heads][s_c]
+  const float* w_in;         // scores before and after, [batch][kv_heads][s_c]
+  float* w_out;
+  int64_t wi_sb, wi_sh, wo_sb, wo_sh;
+};
+constexpr int kRowsMaxSplit = 2048;  // splits of one row, prefix and own together
+
 // Rotary embedding of one layer's q and k heads (rope_kernel).  q/k/qo/ko
 // strides are [B][H][S][D] element strides; cos/sin are [B or 1][S][rot]
 // (c_sb / n_sb = 0 broadcasts one table over the batch).  n_pair = rot / 16
@@ -287,6 +320,8 @@ hipError_t launch_attention_vs(const AttnParams& p, int dtype, int out_dtype, in
 hipError_t launch_vs_build(const VsBuildParams& p, int n_bs, hipStream_t st);
 hipError_t launch_vs_estimate(const VsEstParams& p, int dtype, int D, hipStream_t st);
 hipError_t launch_block_lists(const ListParams& p, hipStream_t st);
+hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,
+                       hipStream_t st);
 hipError_t launch_round(const RoundParams& p, int n, hipStream_t st);
 hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t st);
 

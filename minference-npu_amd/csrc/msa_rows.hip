@@ -1,0 +1,669 @@
+// Attention of a few query rows per kv head against long caches, split over
+// the keys: a batch that shares a prefix, and decode that also leaves the
+// attention weights.
+//
+// shared prefix: row i of sequence b sees every key of the prefix, one cache
+// for all sequences, and its own sequence's keys up to its own position.  The
+// query rows of all sequences and of the query heads of a kv head form one
+// matrix against the prefix, so the prefix is read once per 64 rows instead of
+// once per sequence.
+// decode with accumulation: one query row per head against a cache of lens[b]
+// keys; the raw scores go to the workspace and the second launch adds the
+// normalised weights, summed over the heads of a kv head, to a score per key.
+//
+// A workgroup takes one item: up to 16 MT rows of one kv head against one key
+// range (of the prefix, or of one sequence's own cache), wave w its 32-key
+// blocks w, w + 4, ...
+//   S^T = K . Q^T on the 16-bit 16x16x32 MFMA (exact products, fp32 sums): A
+//     = 16 keys from their rows, B = 16 query rows, held for the whole item.
+//     Lane (lc, lr) gets query lc, keys 4 lr + i of the 16.
+//   O^T += V^T . P^T on the same MFMA, 32 keys a step.  The order of the 32 is
+//     free as long as V and P share it: slot 8 lr + j is key 4 lr + j of the
+//     block's first 16 for j < 4, of the second 16 after that, which is where
+//     P already lies.  V (A operand) is loaded by rows, a lane holding E = D /
+//     16 (8 from D = 128 on) dims of its 8 keys, and pairs of keys are put
+//     together by byte permutes; MFMA e takes dim E lc + e of every lane.
+// No LDS in the loop, and K and V are read once per item.  Softmax statistics
+// and O are fp32; a row's running max moves only when a block exceeds it by
+// 2^kSlack.  P is rounded to the inputs' type twice, P and what that rounding
+// left, so the product's error stays below the output's own rounding.
+// Each item leaves O and (m, l) of its rows in the workspace; the combine
+// kernel merges the items of a row.
+
+#include "msa_common.h"
+#include "msa_kernels.h"
+
+namespace msa {
+
+#define INLINE __attribute__((always_inline))
+
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kSlack = 8.0f;  // P up to 2^8: far inside fp16
+
+template <typename T>
+__device__ inline uint32_t pack2(float a, float b) {
+  if constexpr (T::id == Bf16::id)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+template <typename T>
+__device__ inline float lo_of(uint32_t x) { return T::to_float(uint16_t(x & 0xffffu)); }
+template <typename T>
+__device__ inline float hi_of(uint32_t x) { return T::to_float(uint16_t(x >> 16)); }
+
+// Exponent all ones in either half of a packed pair.
+template <typename T>
+__device__ inline bool any_nonfinite(uint32_t x) {
+  constexpr uint32_t e = T::id == Bf16::id ? 0x7f80u : 0x7c00u;
+  return (x & e) == e || (x & (e << 16)) == (e << 16);
+}
+
+template <int W>
+__device__ inline void load_words(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t soff,
+                                  uint32_t (&w)[W]) {
+  if constexpr (W == 4) {
+    const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, soff, 2));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = x[i];
+  } else if constexpr (W == 3) {
+    const u32x3 x = __builtin_bit_cast(u32x3, __builtin_amdgcn_raw_buffer_load_b96(rs, off, soff, 2));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) w[i] = x[i];
+  } else {
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off, soff, 2));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w[i] = x[i];
+  }
+}
+
+struct Item {
+  const uint16_t* k;  // first key of the item's range
+  const uint16_t* v;
+  uint32_t kss, vss;  // row strides, bytes
+  int n_keys;         // visible keys of the range (0 or less: none)
+  int row0, n_rows;   // rows of the kv head in (sequence, head, position) order
+  int seq_rows;       // rows of one sequence: group * s_q
+  int kvh;
+  int limit;          // CAUSAL: position i sees local keys j <= limit + i
+  int64_t part_row;   // first row of part / ml
+  float* raw;         // SCORES: raw score of (row 0, local key 0)
+  int64_t raw_row;    // SCORES: floats between rows
+};
+
+// Row r of the kv head as an offset into q.
+__device__ inline int64_t q_offset(const RowsParams& P, int kvh, int seq_rows, int r) {
+  const int b = r / seq_rows, rr = r - b * seq_rows;
+  const int g = rr / P.s_q, i = rr - g * P.s_q;
+  return b * P.q_sb + int64_t(kvh * P.group + g) * P.q_sh + int64_t(i) * P.q_ss;
+}
+
+template <int D>
+struct RowsShared {  // merge of an item's waves
+  static constexpr int LP = (D < 128 ? D : 128) + 4;  // padded row
+  __align__(16) float om[4][16][LP];
+  float sm[4][64], sl[4][64];
+};
+
+template <typename T, int D, int MT, bool CAUSAL, bool SCORES>
+__device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh) {
+  constexpr int NKS = D / 32;
+  constexpr int VG = (D + 127) / 128;       // groups of 128 dims of V
+  constexpr int E = D < 128 ? D / 16 : 8;   // dims of a lane in a group
+  constexpr int W = E / 2;
+  constexpr int DG = 16 * E;                // dims of a group
+  auto& om = sh.om;
+  auto& sm = sh.sm;
+  auto& sl = sh.sl;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int lr = lane >> 4;
+  const int lc = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  if (it.n_keys <= 0) {  // nothing visible: an empty split
+    for (int r = tid; r < it.n_rows; r += 256) {
+      P.ml[2 * (it.part_row + r)] = -__builtin_inff();
+      P.ml[2 * (it.part_row + r) + 1] = 0.0f;
+    }
+    return;
+  }
+
+  // query rows as the QK B operand: lane (lc, lr) holds dims 32 ks + 8 lr .. +7
+  // of row lc (rows past n_rows repeat the last one and are not stored)
+  u32x4 qb[MT][NKS];
+  int lim[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = it.row0 + min(16 * mt + lc, it.n_rows - 1);
+    const uint16_t* qrow =
+        reinterpret_cast<const uint16_t*>(P.q) + q_offset(P, it.kvh, it.seq_rows, r);
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) qb[mt][ks] = load16(qrow + 32 * ks + 8 * lr);
+    lim[mt] = CAUSAL ? it.limit + r % P.s_q : 0;
+  }
+
+  // Buffer descriptors end with the last visible key, so rows behind it,
+  // whatever they hold, read 0.
+  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(it.k), short(0), int(uint32_t(it.n_keys - 1) * it.kss + 2 * D), 0x00020000);
+  const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(it.v), short(0), int(uint32_t(it.n_keys - 1) * it.vss + 2 * D), 0x00020000);
+  uint32_t koff[2], voff[8];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) koff[u] = uint32_t(16 * u + lc) * it.kss + 16u * lr;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    voff[j] = uint32_t(16 * (j >> 2) + 4 * lr + (j & 3)) * it.vss + 2u * E * lc;
+
+  // The scalar offset names the block's first key, which is visible: the
+  // range check compares the lane offset with the records left behind it.
+  auto load_block = [&](int j0, u32x4 (&kr)[2][NKS], uint32_t (&vr)[8][VG][W]) INLINE {
+    const uint32_t ks0 = uint32_t(j0) * it.kss, vs0 = uint32_t(j0) * it.vss;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks)
+        kr[u][ks] = __builtin_bit_cast(
+            u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, koff[u] + 64 * ks, ks0, 2));
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int g = 0; g < VG; ++g) load_words<W>(vrs, voff[j] + 256 * g, vs0, vr[j][g]);
+  };
+
+  // o[mt][g][e]: lane (lc, lr) holds row lc, dims 128 g + E (4 lr + j) + e
+  f32x4 o[MT][VG][E];
+  float m[MT], mp[MT], l[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = -__builtin_inff();  // running max, raw scores times c, the same in a row's 4 lanes
+    mp[mt] = 0.0f;              // what P is taken against: m, or 0 without a score above -inf
+    l[mt] = 0.0f;               // this lane's share of the sum
+#pragma unroll
+    for (int g = 0; g < VG; ++g)
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[mt][g][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const float c = P.scale_log2;
+
+  auto block = [&](int j0, const u32x4 (&kr)[2][NKS], uint32_t (&vr)[8][VG][W]) INLINE {
+    const bool edge = CAUSAL ? j0 + 31 > it.limit : j0 + 32 > it.n_keys;
+    u32x4 ph[MT], pl[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      f32x4 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) s[u] = mfma_qk<T>(kr[u][ks], qb[mt][ks], s[u]);
+      }
+      if (SCORES && lc < it.n_rows) {  // MT == 1
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = j0 + 16 * u + 4 * lr + i;
+            if (j < it.n_keys) it.raw[lc * it.raw_row + j] = s[u][i];
+          }
+      }
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = j0 + 16 * u + 4 * lr + i;
+            if (CAUSAL ? j > lim[mt] || j >= it.n_keys : j >= it.n_keys) s[u][i] = -__builtin_inff();
+          }
+      }
+      float bm = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * c;
+      if (__ballot(bm > m[mt] + kSlack) != 0) {
+        const float mn = fmaxf(m[mt], bm);
+        mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(m[mt] - mp[mt]);  // m = -inf at first: 0
+        m[mt] = mn;
+        l[mt] *= al;
+#pragma unroll
+        for (int g = 0; g < VG; ++g)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[mt][g][e] *= al;
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], c, -mp[mt]));
+        l[mt] += p[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ph[mt][j] = pack2<T>(p[2 * j], p[2 * j + 1]);
+        pl[mt][j] = pack2<T>(p[2 * j] - lo_of<T>(ph[mt][j]), p[2 * j + 1] - hi_of<T>(ph[mt][j]));
+      }
+    }
+    if (CAUSAL && edge) {
+      // A key that some rows see and others do not: a zero P times an Inf or
+      // NaN of its V would reach the others.  Such values leave the product
+      // and are added one key at a time, to the rows that see it.
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int g = 0; g < VG; ++g)
+#pragma unroll
+          for (int x = 0; x < W; ++x) bad |= any_nonfinite<T>(vr[j][g][x]);
+      if (__ballot(bad) != 0) {
+        constexpr uint32_t ex = T::id == Bf16::id ? 0x7f80u : 0x7c00u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int g = 0; g < VG; ++g)
+#pragma unroll
+            for (int x = 0; x < W; ++x) {
+              if ((vr[j][g][x] & ex) == ex) vr[j][g][x] &= 0xffff0000u;
+              if ((vr[j][g][x] & (ex << 16)) == (ex << 16)) vr[j][g][x] &= 0xffffu;
+            }
+        for (int kk = 0; kk < 32 && j0 + kk < it.n_keys; ++kk) {
+          const uint16_t* vrow = it.v + int64_t(j0 + kk) * (it.vss / 2);
+          const int slot = 4 * (kk >> 4) + (kk & 3);  // P's place in its lane
+          const int src = lc + 16 * ((kk & 15) >> 2);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t hw = 0, lw = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if ((slot >> 1) == x) {
+                hw = ph[mt][x];
+                lw = pl[mt][x];
+              }
+            const float pv = (slot & 1) ? hi_of<T>(hw) + hi_of<T>(lw) : lo_of<T>(hw) + lo_of<T>(lw);
+            const float pk = __shfl(pv, src, 64);
+            const bool sees = j0 + kk <= lim[mt];
+#pragma unroll
+            for (int g = 0; g < VG; ++g)
+#pragma unroll
+              for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float x = T::to_float(vrow[128 * g + E * (4 * lr + i) + e]);
+                  if (sees && !__builtin_isfinite(x)) o[mt][g][e][i] += pk * x;
+                }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < VG; ++g)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        u32x4 a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          a[j] = __builtin_amdgcn_perm(vr[2 * j + 1][g][e >> 1], vr[2 * j][g][e >> 1],
+                                       e & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          o[mt][g][e] = mfma_qk<T>(a, ph[mt], o[mt][g][e]);
+          o[mt][g][e] = mfma_qk<T>(a, pl[mt], o[mt][g][e]);
+        }
+      }
+  };
+
+  // Wave w takes blocks first + 128 i, i < nblk, in two register sets; loads
+  // past the wave's last block repeat it, so every load is unconditional.
+  const int first = 32 * w;
+  const int nblk = it.n_keys > first ? (it.n_keys - first + 127) / 128 : 0;
+  auto jb = [&](int i) { return first + 128 * min(i, nblk - 1); };
+  if constexpr (D > 256) {  // one register set: q, O, K and V of a block fill the file
+    for (int i = 0; i < nblk; ++i) {
+      u32x4 ka[2][NKS];
+      uint32_t va[8][VG][W];
+      load_block(jb(i), ka, va);
+      block(jb(i), ka, va);
+    }
+  } else if (nblk > 0) {
+    u32x4 ka[2][NKS], kb[2][NKS];
+    uint32_t va[8][VG][W], vb[8][VG][W];
+    load_block(jb(0), ka, va);
+    for (int i = 0; i < nblk; i += 2) {
+      load_block(jb(i + 1), kb, vb);
+      block(jb(i), ka, va);
+      if (i + 1 >= nblk) break;
+      load_block(jb(i + 2), ka, va);
+      block(jb(i + 1), kb, vb);
+    }
+  }
+
+  // ---- merge the 4 waves, 16 rows and a group of dims at a time
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    l[mt] += __shfl_xor(l[mt], 16, 64);
+    l[mt] += __shfl_xor(l[mt], 32, 64);
+    if (lr == 0) {
+      sm[w][16 * mt + lc] = m[mt];
+      sl[w][16 * mt + lc] = l[mt];
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    if (16 * mt >= it.n_rows) break;
+#pragma unroll
+    for (int g = 0; g < VG; ++g) {
+      if (mt + g > 0) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+          *reinterpret_cast<float2*>(&om[w][lc][E * (4 * lr + i) + e]) =
+              make_float2(o[mt][g][e][i], o[mt][g][e + 1][i]);
+      __syncthreads();
+      for (int x = tid; x < 16 * (DG / 4); x += 256) {
+        const int row = x / (DG / 4), d = 4 * (x - row * (DG / 4));
+        if (16 * mt + row >= it.n_rows) continue;
+        float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) M = fmaxf(M, sm[v][16 * mt + row]);
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float mv = sm[v][16 * mt + row];
+          if (mv == -__builtin_inff()) continue;
+          const float f = __builtin_amdgcn_exp2f(mv - M);
+          L += f * sl[v][16 * mt + row];
+          const float4 y = *reinterpret_cast<const float4*>(&om[v][row][d]);
+          acc.x = __builtin_fmaf(f, y.x, acc.x);
+          acc.y = __builtin_fmaf(f, y.y, acc.y);
+          acc.z = __builtin_fmaf(f, y.z, acc.z);
+          acc.w = __builtin_fmaf(f, y.w, acc.w);
+        }
+        const int64_t pr = it.part_row + 16 * mt + row;
+        *reinterpret_cast<float4*>(P.part + pr * D + 128 * g + d) = acc;
+        if (g == 0 && d == 0) {
+          P.ml[2 * pr] = M;
+          P.ml[2 * pr + 1] = L;
+        }
+      }
+    }
+  }
+}
+
+__device__ inline int clamped_len(const RowsParams& P, int b) {
+  return P.lens ? max(0, min(P.lens[b], P.s_c)) : P.s_c;
+}
+
+// Item blockIdx.x: the prefix items first ((kv head, key range), row tile),
+// then the own-cache items ((sequence, kv head), key range, row tile).
+template <typename T, int D, int MTP, int MTO, bool CAUSAL, bool SCORES>
+__global__ __launch_bounds__(256) void rows_kernel(const RowsParams P) {
+  __shared__ RowsShared<D> sh;
+  Item it;
+  it.seq_rows = P.group * P.s_q;
+  it.raw = nullptr;
+  it.raw_row = 0;
+  int x = blockIdx.x;
+  if (MTP > 0 && x < P.n_prefix_items) {
+    const int rt = x % P.n_rt;
+    x /= P.n_rt;
+    const int split = x % P.n_sp;
+    it.kvh = x / P.n_sp;
+    const int R = P.batch * it.seq_rows;
+    const int j0 = split * P.chunk_p;
+    it.k = reinterpret_cast<const uint16_t*>(P.kp) + it.kvh * P.kp_sh + int64_t(j0) * P.kp_ss;
+    it.v = reinterpret_cast<const uint16_t*>(P.vp) + it.kvh * P.vp_sh + int64_t(j0) * P.vp_ss;
+    it.kss = uint32_t(P.kp_ss) * 2u;
+    it.vss = uint32_t(P.vp_ss) * 2u;
+    it.n_keys = min(P.chunk_p, P.s_p - j0);
+    it.limit = 0;
+    it.row0 = rt * 16 * MTP;
+    it.n_rows = min(16 * MTP, R - it.row0);
+    it.part_row = (int64_t(it.kvh) * P.n_sp + split) * R + it.row0;
+    if constexpr (MTP > 0) rows_item<T, D, MTP, false, false>(P, it, sh);
+    return;
+  }
+  x -= P.n_prefix_items;
+  const int rt = x % P.n_rto;
+  x /= P.n_rto;
+  const int split = x % P.n_so;
+  x /= P.n_so;
+  it.kvh = x % P.kv_heads;
+  const int b = x / P.kv_heads;
+  const int j0 = split * P.chunk_o;
+  const int len = clamped_len(P, b);
+  it.k = reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + it.kvh * P.k_sh + int64_t(j0) * P.k_ss;
+  it.v = reinterpret_cast<const uint16_t*>(P.v) + b * P.v_sb + it.kvh * P.v_sh + int64_t(j0) * P.v_ss;
+  it.kss = uint32_t(P.k_ss) * 2u;
+  it.vss = uint32_t(P.v_ss) * 2u;
+  it.n_keys = min(P.chunk_o, len - j0);
+  it.limit = len - P.s_q - j0;
+  const int r0 = rt * 16 * MTO;
+  it.row0 = b * it.seq_rows + r0;
+  it.n_rows = min(16 * MTO, it.seq_rows - r0);
+  it.part_row = P.own_row0 + (int64_t(b * P.kv_heads + it.kvh) * P.n_so + split) * it.seq_rows + r0;
+  if constexpr (SCORES) {  // s_q == 1: rows are the heads of the group
+    it.raw_row = P.s_c;
+    it.raw = P.raw + (int64_t(b) * P.heads + it.kvh * P.group + r0) * P.s_c + j0;
+  }
+  rows_item<T, D, MTO, CAUSAL, SCORES>(P, it, sh);
+}
+
+template <typename T, bool OUT_F32>
+__device__ inline void store_one(void* o, int64_t off, float r) {
+  if constexpr (OUT_F32) {
+    reinterpret_cast<float*>(o)[off] = r;
+  } else {
+    reinterpret_cast<uint16_t*>(o)[off] = T::from_float(r);
+  }
+}
+
+// Place in part / ml of split s of row rr of (sequence b, kv head kvh): the
+// prefix splits first, then the own cache's.
+__device__ inline int64_t part_row_of(const RowsParams& P, int b, int kvh, int rr, int s) {
+  const int seq_rows = P.group * P.s_q;
+  if (s < P.n_sp)
+    return (int64_t(kvh) * P.n_sp + s) * P.batch * seq_rows + int64_t(b) * seq_rows + rr;
+  return P.own_row0 + (int64_t(b * P.kv_heads + kvh) * P.n_so + (s - P.n_sp)) * seq_rows + rr;
+}
+
+// Output row rr of (b, kvh): O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s
+// over its splits, by one workgroup.  Splits without a score above -inf leave
+// no O.
+template <typename T, bool OUT_F32, int D>
+__device__ void combine_row(const RowsParams& P, int b, int kvh, int rr) {
+  constexpr int TPR = D / 4;    // threads per split row, 4 elements each
+  constexpr int G = 256 / TPR;  // split groups
+  __shared__ float fs[kRowsMaxSplit];
+  __shared__ float red[8];
+  __shared__ __align__(16) float acc_g[G][D];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int ns = P.n_sp + P.n_so;
+  float mx = -__builtin_inff();
+  for (int s = tid; s < ns; s += 256) {
+    const float ms = P.ml[2 * part_row_of(P, b, kvh, rr, s)];
+    fs[s] = ms;
+    mx = fmaxf(mx, ms);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  if (lane == 0) red[w] = mx;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float L = 0.0f;
+  for (int s = tid; s < ns; s += 256) {
+    const float ms = fs[s];
+    const float f = ms == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
+    fs[s] = f;
+    L += f * P.ml[2 * part_row_of(P, b, kvh, rr, s) + 1];
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
+  if (lane == 0) red[4 + w] = L;
+  __syncthreads();
+  L = (red[4] + red[5]) + (red[6] + red[7]);
+
+  const int g = tid / TPR, c = tid - g * TPR;
+  if (g < G) {
+    float a0 = 0.0f, a1 = 0.0f, a2 = 0.0f, a3 = 0.0f;
+    for (int s = g; s < ns; s += G) {
+      const float f = fs[s];
+      if (f == 0.0f) continue;
+      const float4 x = *reinterpret_cast<const float4*>(P.part + part_row_of(P, b, kvh, rr, s) * D + 4 * c);
+      a0 = __builtin_fmaf(f, x.x, a0);
+      a1 = __builtin_fmaf(f, x.y, a1);
+      a2 = __builtin_fmaf(f, x.z, a2);
+      a3 = __builtin_fmaf(f, x.w, a3);
+    }
+    *reinterpret_cast<float4*>(&acc_g[g][4 * c]) = float4{a0, a1, a2, a3};
+  }
+  __syncthreads();
+  const int hg = rr / P.s_q, i = rr - hg * P.s_q;
+  const int64_t off = b * P.o_sb + int64_t(kvh * P.group + hg) * P.o_sh + int64_t(i) * P.o_ss;
+  for (int d = tid; d < D; d += 256) {
+    float acc = 0.0f;
+#pragma unroll
+    for (int q = 0; q < G; ++q) acc += acc_g[q][d];
+    // no score above -inf: 0; l = NaN (a NaN or +inf score) stays NaN
+    store_one<T, OUT_F32>(P.o, off + d, L == 0.0f ? 0.0f : acc / L);
+  }
+}
+
+template <typename T, bool OUT_F32, int D>
+__global__ __launch_bounds__(256) void rows_combine_kernel(const RowsParams P) {
+  const int seq_rows = P.group * P.s_q;
+  int x = blockIdx.x;
+  const int rr = x % seq_rows;
+  x /= seq_rows;
+  combine_row<T, OUT_F32, D>(P, x / P.kv_heads, x % P.kv_heads, rr);
+}
+
+constexpr int kWeightKeys = 1024;  // keys of a weight workgroup, 4 per thread
+
+// Second launch of decode_accumulate, grid (key blocks + group, B * kv heads):
+// the first key blocks add the weights of kWeightKeys keys, the others merge
+// one head's output each.
+template <typename T, bool OUT_F32, int D>
+__global__ __launch_bounds__(256) void rows_weights_kernel(const RowsParams P, int n_kb) {
+  __shared__ float sM[kMaxHeads], sR[kMaxHeads];
+  const int b = blockIdx.y / P.kv_heads, kvh = blockIdx.y % P.kv_heads;
+  if (int(blockIdx.x) >= n_kb) {
+    combine_row<T, OUT_F32, D>(P, b, kvh, int(blockIdx.x) - n_kb);
+    return;
+  }
+  const int len = clamped_len(P, b);
+  const int j0 = int(blockIdx.x) * kWeightKeys;
+  if (j0 >= len) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  for (int g = w; g < P.group; g += 4) {  // (M, 1 / L) of each head
+    float M = -__builtin_inff();
+    for (int s = lane; s < P.n_so; s += 64) M = fmaxf(M, P.ml[2 * part_row_of(P, b, kvh, g, s)]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
+    float L = 0.0f;
+    for (int s = lane; s < P.n_so; s += 64) {
+      const int64_t pr = part_row_of(P, b, kvh, g, s);
+      const float ms = P.ml[2 * pr];
+      if (ms != -__builtin_inff()) L += __builtin_amdgcn_exp2f(ms - M) * P.ml[2 * pr + 1];
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
+    if (lane == 0) {
+      sM[g] = M == -__builtin_inff() ? 0.0f : M;
+      sR[g] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+  }
+  __syncthreads();
+  const float* raw = P.raw + (int64_t(b) * P.heads + kvh * P.group) * P.s_c;
+  const float* in = P.w_in + b * P.wi_sb + kvh * P.wi_sh;
+  float* out = P.w_out + b * P.wo_sb + kvh * P.wo_sh;
+#pragma unroll
+  for (int q = 0; q < kWeightKeys / 256; ++q) {
+    const int j = j0 + 256 * q + tid;
+    if (j >= len) break;
+    float acc = 0.0f;
+    for (int g = 0; g < P.group; ++g)
+      acc += sR[g] * __builtin_amdgcn_exp2f(
+                         __builtin_fmaf(raw[int64_t(g) * P.s_c + j], P.scale_log2, -sM[g]));
+    out[j] = in[j] + acc;
+  }
+}
+
+template <typename T, bool OUT_F32, int D, int MTP, int MTO, bool CAUSAL>
+hipError_t launch_prefix_k(const RowsParams& p, hipStream_t st) {
+  if (p.n_items > 0) {
+    hipLaunchKernelGGL((rows_kernel<T, D, MTP, MTO, CAUSAL, false>), dim3(p.n_items), dim3(256), 0,
+                       st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((rows_combine_kernel<T, OUT_F32, D>),
+                     dim3(p.batch * p.heads * p.s_q), dim3(256), 0, st, p);
+  return hipGetLastError();
+}
+
+template <typename T, bool OUT_F32, int D>
+hipError_t launch_prefix_d(const RowsParams& p, hipStream_t st) {
+  if constexpr (D <= 128) {
+    if (p.s_q == 1)
+      return p.mt == 4   ? launch_prefix_k<T, OUT_F32, D, 4, 1, false>(p, st)
+             : p.mt == 2 ? launch_prefix_k<T, OUT_F32, D, 2, 1, false>(p, st)
+                         : launch_prefix_k<T, OUT_F32, D, 1, 1, false>(p, st);
+    return p.mt == 4   ? launch_prefix_k<T, OUT_F32, D, 4, 1, true>(p, st)
+           : p.mt == 2 ? launch_prefix_k<T, OUT_F32, D, 2, 1, true>(p, st)
+                       : launch_prefix_k<T, OUT_F32, D, 1, 1, true>(p, st);
+  } else {
+    return p.s_q == 1 ? launch_prefix_k<T, OUT_F32, D, 1, 1, false>(p, st)
+                      : launch_prefix_k<T, OUT_F32, D, 1, 1, true>(p, st);
+  }
+}
+
+template <typename T, bool OUT_F32, int D>
+hipError_t launch_accumulate_d(const RowsParams& p, hipStream_t st) {
+  if (p.n_items > 0) {
+    hipLaunchKernelGGL((rows_kernel<T, D, 0, 1, false, true>), dim3(p.n_items), dim3(256), 0, st, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  const int n_kb = (p.s_c + kWeightKeys - 1) / kWeightKeys;
+  hipLaunchKernelGGL((rows_weights_kernel<T, OUT_F32, D>),
+                     dim3(n_kb + p.group, p.batch * p.kv_heads), dim3(256), 0, st, p, n_kb);
+  return hipGetLastError();
+}
+
+template <typename T, bool OUT_F32>
+hipError_t launch_rows_t(const RowsParams& p, bool accumulate, int D, hipStream_t st) {
+#define MSA_ROWS_D(DD)                                                      \
+  if (D == DD)                                                              \
+    return accumulate ? launch_accumulate_d<T, OUT_F32, DD>(p, st)          \
+                      : launch_prefix_d<T, OUT_F32, DD>(p, st);
+  MSA_ROWS_D(64)
+  MSA_ROWS_D(96)
+  MSA_ROWS_D(128)
+  MSA_ROWS_D(256)
+  MSA_ROWS_D(512)
+#undef MSA_ROWS_D
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,
+                       hipStream_t st) {
+  const bool f32 = out_dtype == 3;
+  if (dtype == Bf16::id)
+    return f32 ? launch_rows_t<Bf16, true>(p, accumulate, D, st)
+               : launch_rows_t<Bf16, false>(p, accumulate, D, st);
+  return f32 ? launch_rows_t<F16, true>(p, accumulate, D, st)
+             : launch_rows_t<F16, false>(p, accumulate, D, st);
+}
+
+}  // namespace msa

@@ -2,7 +2,8 @@
 
 Same public names as the reference package (MInference-NPU/minference/__init__.py:8-44):
 MInference, MInferenceConfig, minference_patch, patch_hf, get_support_models,
-block_sparse_attention, streaming_forward; plus dense_attention.
+block_sparse_attention, streaming_forward; plus dense_attention and the cache
+operators (shared_prefix_attention, decode_accumulate).
 """
 
 from .configs.model2path import get_support_models
@@ -17,6 +18,8 @@ __all__ = [
     "block_sparse_attention",
     "streaming_forward",
     "dense_attention",
+    "shared_prefix_attention",
+    "decode_accumulate",
 ]
 
 
@@ -49,4 +52,8 @@ def __getattr__(name):
         from .backend.attention import dense_attention
 
         return dense_attention
+    if name in ("shared_prefix_attention", "decode_accumulate"):
+        from .backend import cached
+
+        return getattr(cached, name)
     raise AttributeError(name)

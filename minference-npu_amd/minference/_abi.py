@@ -55,7 +55,7 @@ MSA_ESTIMATE_SELECT_ONLY = 8
 
 MSA_MAX_HEADS = 128
 MSA_BLOCK = 64
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _DTYPE_CODE = {
     torch.bfloat16: MSA_DTYPE_BF16,
@@ -87,6 +87,10 @@ EXPORTED_SYMBOLS = (
     "msa_block_lists",
     "msa_split_workspace_bytes",
     "msa_layer_attention_split",
+    "msa_shared_prefix_workspace_bytes",
+    "msa_shared_prefix_attention",
+    "msa_decode_accumulate_workspace_bytes",
+    "msa_decode_accumulate",
 )
 
 
@@ -278,6 +282,19 @@ def load_library() -> ctypes.CDLL:
             ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32,
             ctypes.c_void_p,
         ]
+        T4 = ctypes.POINTER(MsaTensor4)
+        lib.msa_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
+        lib.msa_shared_prefix_workspace_bytes.argtypes = [T4] * 5
+        lib.msa_shared_prefix_attention.restype = ctypes.c_int
+        lib.msa_shared_prefix_attention.argtypes = [T4] * 6 + [
+            ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
+        ]
+        lib.msa_decode_accumulate_workspace_bytes.restype = ctypes.c_size_t
+        lib.msa_decode_accumulate_workspace_bytes.argtypes = [T4] * 3
+        lib.msa_decode_accumulate.restype = ctypes.c_int
+        lib.msa_decode_accumulate.argtypes = [T4] * 4 + [ctypes.c_void_p, T4, T4] + [
+            ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
+        ]
         ver = lib.msa_abi_version()
         if ver != ABI_VERSION:
             raise ImportError(f"libmsa ABI version {ver} != expected {ABI_VERSION}")
@@ -361,6 +378,47 @@ def decode_attention_noalloc(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     check(load_library().msa_decode_attention_noalloc(
         ctypes.byref(qd), ctypes.byref(kd), ctypes.byref(vd), ctypes.byref(od), float(scale),
         current_stream_handle(q.device)))
+
+
+def _lens_ptr(lens: Optional[torch.Tensor], batch: int, device: torch.device) -> Optional[int]:
+    if lens is None:
+        return None
+    if (lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous()
+            or lens.device != device):
+        raise ValueError(f"lens must be a contiguous int32 [{batch}] tensor on q's device, got "
+                         f"{tuple(lens.shape)} {lens.dtype} on {lens.device}")
+    return lens.data_ptr()
+
+
+def shared_prefix_attention(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, out: torch.Tensor, lens: Optional[torch.Tensor],
+                            scale: float) -> None:
+    """Launch msa_shared_prefix_attention on the current stream of q's device:
+    q [B,H,S_q,D] against the prefix kp/vp [1,H_kv,S_p,D] and the own caches
+    k/v [B,H_kv,S_c,D]."""
+    lib = load_library()
+    lens_p = _lens_ptr(lens, q.shape[0], q.device)
+    ds = [ctypes.byref(tensor4(t)) for t in (q, kp, vp, k, v, out)]
+    with torch.cuda.device(q.device):
+        ws = workspace(lib.msa_shared_prefix_workspace_bytes(*ds[:5]), q.device)
+        check(lib.msa_shared_prefix_attention(*ds, lens_p, float(scale), ws.data_ptr(), ws.numel(),
+                                              current_stream_handle(q.device)))
+
+
+def decode_accumulate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                      lens: Optional[torch.Tensor], scores: torch.Tensor,
+                      scores_out: torch.Tensor, scale: float) -> None:
+    """Launch msa_decode_accumulate on the current stream of q's device: q
+    [B,H,1,D] against the cache k/v; scores and scores_out fp32 [B,H_kv,S]."""
+    lib = load_library()
+    lens_p = _lens_ptr(lens, q.shape[0], q.device)
+    qd, kd, vd, od, sd, rd = (ctypes.byref(tensor4(t)) for t in (
+        q, k, v, out, scores.unsqueeze(-1), scores_out.unsqueeze(-1)))
+    with torch.cuda.device(q.device):
+        ws = workspace(lib.msa_decode_accumulate_workspace_bytes(qd, kd, vd), q.device)
+        check(lib.msa_decode_accumulate(qd, kd, vd, od, lens_p, sd, rd, float(scale),
+                                        ws.data_ptr(), ws.numel(),
+                                        current_stream_handle(q.device)))
 
 
 def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

@@ -1,0 +1,165 @@
+"""Attention over caches that a batch shares or that are about to be cut.
+
+``shared_prefix_attention``: the sequences of a batch continue one prefix,
+whose cache is held once and read once for all of them.  ``decode_accumulate``:
+one query row per head, as decode_dense (reference
+minference/backend_npu/attention.py:274-314), which also adds the attention
+weights to a running score per key, the scores ``evict_kv_cache`` cuts a cache
+by.  The reference has neither: it keeps one full cache per sequence.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _abi
+from ..ops.common import (SUPPORTED_DTYPES, accepts_float32, check_written, dense_scale,
+                          kernel_head_dim, kernel_view, make_out, pad_head_dim)
+
+__all__ = ["shared_prefix_attention", "decode_accumulate"]
+
+
+def _check_caches(q: torch.Tensor, pairs) -> None:
+    """Shapes, types and devices of (name, k, v, batch) cache pairs against q."""
+    if q.dim() != 4:
+        raise ValueError(f"q must be 4-D [B,H,S,D], got {q.dim()}-D")
+    tensors = [q]
+    for name, k, v, batch in pairs:
+        if k.dim() != 4 or v.shape != k.shape:
+            raise ValueError(f"k and v of the {name} must be 4-D [B,H_kv,S,D] of one shape, got "
+                             f"{tuple(k.shape)} and {tuple(v.shape)}")
+        if k.shape[0] != batch or k.shape[3] != q.shape[3]:
+            raise ValueError(f"the {name} must be [{batch},H_kv,S,{q.shape[3]}] for q "
+                             f"{tuple(q.shape)}, got {tuple(k.shape)}")
+        if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+            raise ValueError(f"q heads {q.shape[1]} not a multiple of {name} heads {k.shape[1]}")
+        tensors += [k, v]
+    if len({p[1].shape[1] for p in pairs}) != 1:
+        raise ValueError("prefix and own caches must have the same kv heads")
+    _abi.require_device(*tensors)
+    for t in tensors:
+        if t.dtype not in SUPPORTED_DTYPES:
+            raise NotImplementedError(f"the MI355X kernels take bf16 or fp16 inputs, got {t.dtype}")
+        if t.dtype != q.dtype:
+            raise ValueError("q, k and v must share one dtype")
+    if q.shape[3] < 1:
+        raise ValueError("head_dim must be positive")
+
+
+def _padded(ts, out: torch.Tensor, fn) -> None:
+    """fn(views of ts, out) at the kernel head dim of ts[0]; other head dims
+    are zero-padded to it (no dot product changes) and cut again."""
+    d = ts[0].shape[3]
+    dk = kernel_head_dim(d)
+    if dk == d:
+        fn([kernel_view(t) for t in ts], out)
+        return
+    tmp = torch.empty((*out.shape[:3], dk), dtype=out.dtype, device=out.device)
+    fn([pad_head_dim(t, dk) for t in ts], tmp)
+    out.copy_(tmp[..., :d])
+
+
+@accepts_float32(("q", "k_prefix", "v_prefix", "k_cache", "v_cache"))
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k_prefix: torch.Tensor,
+    v_prefix: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    *,
+    lens: Optional[torch.Tensor] = None,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of a batch whose sequences continue one shared prefix.
+
+    Args:
+        q: ``[B, H, S_q, D]``, the last S_q tokens of each sequence (1 for
+            decode; a short question or drafted tokens otherwise).
+        k_prefix, v_prefix: ``[1, H_kv, S_p, D]``, seen by every row;
+            ``H % H_kv == 0``; S_p may be 0.
+        k_cache, v_cache: ``[B, H_kv, S_c, D]``, each sequence's own keys after
+            the prefix, the queries' own among them; S_c may be 0.
+        lens: int32 ``[B]`` on the device, keys of each own cache in use (None:
+            S_c; values are clamped to [0, S_c]).  Row i sees own keys
+            ``j <= lens[b] - S_q + i``.  Keys behind lens[b] are not used,
+            whatever they hold.
+        scale: 1/sqrt(D) by default.
+        out: q's shape, q's dtype or fp32.
+
+    The prefix is read once per 64 query rows (batch x heads of a kv head x
+    S_q), not once per sequence.  Equal to dense attention over the
+    concatenated caches.  A row that sees no key, or only scores of -inf, is 0.
+    """
+    _check_caches(q, [("prefix", k_prefix, v_prefix, 1), ("own cache", k_cache, v_cache, q.shape[0])])
+    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
+    result = make_out(q, out)
+    if out is not None:
+        check_written("out", out)
+    if q.numel() == 0:
+        return result
+    _padded((q, k_prefix, v_prefix, k_cache, v_cache), result,
+            lambda ts, r: _abi.shared_prefix_attention(*ts, r, lens, s))
+    return result
+
+
+def _check_scores(name: str, t: torch.Tensor, k_cache: torch.Tensor) -> None:
+    if tuple(t.shape) != tuple(k_cache.shape[:3]) or t.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 {tuple(k_cache.shape[:3])}, got {t.dtype} "
+                         f"{tuple(t.shape)}")
+    if t.device != k_cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name} must be contiguous over the keys")
+
+
+@accepts_float32(("q", "k_cache", "v_cache"), once=True)
+def decode_accumulate(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    scores: torch.Tensor,
+    *,
+    lens: Optional[torch.Tensor] = None,
+    scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    scores_out: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """decode_dense over a ragged batch, with the attention weights added to a
+    score per key: ``scores_out[b, g, j] = scores[b, g, j] + sum of the weights
+    that the heads of kv head g give key j``, j < lens[b].
+
+    Args:
+        q: ``[B, H, 1, D]``; k_cache, v_cache: ``[B, H_kv, S, D]``.
+        scores: float32 ``[B, H_kv, S]``, contiguous over the keys.
+        lens: int32 ``[B]`` on the device, keys in use (None: S; values are
+            clamped to [0, S]).  Keys behind are not used, whatever they hold,
+            and their scores are left as they are.
+        scale: 1/sqrt(D) by default.
+        out: q's shape, q's dtype or fp32.
+        scores_out: where the sums go; ``scores`` itself by default.
+
+    Returns (out, scores_out).  The same call gives the same bits.  With lens[b]
+    = 0, or only scores of -inf, a row is 0 and adds nothing.
+    """
+    _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
+    if q.shape[2] != 1:
+        raise NotImplementedError("decode_accumulate takes one query row")
+    _check_scores("scores", scores, k_cache)
+    if scores_out is None:
+        scores_out = scores
+    else:
+        _check_scores("scores_out", scores_out, k_cache)
+    same = scores_out.data_ptr() == scores.data_ptr() and scores_out.stride() == scores.stride()
+    check_written("scores_out", scores_out, () if same else (("scores", scores),))
+    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
+    result = make_out(q, out)
+    if out is not None:
+        check_written("out", out)
+    if q.numel() == 0:
+        return result, scores_out
+    _padded((q, k_cache, v_cache), result,
+            lambda ts, r: _abi.decode_accumulate(*ts, r, lens, scores, scores_out, s))
+    return result, scores_out

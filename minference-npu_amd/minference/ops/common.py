@@ -50,7 +50,7 @@ def _long_op(ts: Sequence[torch.Tensor], causal: bool) -> bool:
     return 4 * q.shape[0] * q.shape[1] * q.shape[3] * pairs >= 2 ** 37
 
 
-def accepts_float32(names: Sequence[str], has_out: bool = True):
+def accepts_float32(names: Sequence[str], has_out: bool = True, once: bool = False):
     """Decorator for the public ops: called with float32 tensors ``names``,
     the op runs on their on-device roundings to sixteen_bit_dtype and, when
     it has an output, writes it in float32 (``out`` must then be float32 or
@@ -58,7 +58,9 @@ def accepts_float32(names: Sequence[str], has_out: bool = True):
     fp32 (minference/ops/streaming_kernel_npu.py:138-144,
     minference/ops/block_sparse_kernel_npu.py:340-348); here float32 inputs
     get the 16-bit kernels' arithmetic on their roundings.  Inputs of other
-    dtypes go to the op unchanged (bf16 / fp16, or its dtype error).
+    dtypes go to the op unchanged (bf16 / fp16, or its dtype error).  ``once``:
+    the op updates a tensor in place, so it may not run twice and waits for
+    the range check.
     GPU tensors that msa_round_f32 takes are rounded and range-checked by that
     one launch, others by torch ops."""
 
@@ -92,7 +94,7 @@ def accepts_float32(names: Sequence[str], has_out: bool = True):
             # the check fails; a long one, and one whose output overwrites an
             # input, waits for the check first and runs once
             out = ba.arguments.get("out")
-            wait = _long_op(ts, ba.arguments.get("causal", True)) or has_out and any(
+            wait = once or _long_op(ts, ba.arguments.get("causal", True)) or has_out and any(
                 out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr() for t in ts)
             flag = torch.zeros(1, dtype=torch.int32, pin_memory=True)
             checked = torch.cuda.Event()
@@ -246,6 +248,32 @@ def make_out(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     if out.device != q.device:
         raise ValueError("out must be on q's device")
     return out
+
+
+def _span(t: torch.Tensor):
+    """First and last byte of t's elements (t not empty)."""
+    a = t.data_ptr()
+    return a, a + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) - 1
+
+
+def check_written(name: str, t: torch.Tensor, others=()) -> None:
+    """An output tensor's elements lie apart from each other and from the
+    (name, tensor) ``others``."""
+    if t.numel() == 0:
+        return
+    inner = 1
+    for st, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if st < inner:
+            raise ValueError(f"{name} has elements that share memory (shape {tuple(t.shape)}, "
+                             f"strides {t.stride()})")
+        inner = st * (n - 1) + inner
+    lo, hi = _span(t)
+    for other, u in others:
+        if u.numel() == 0:
+            continue
+        ulo, uhi = _span(u)
+        if lo <= uhi and ulo <= hi:
+            raise ValueError(f"{name} shares memory with {other}")
 
 
 def head_chunks(n_heads: int):
