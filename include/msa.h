@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define MSA_ABI_VERSION 16
+#define MSA_ABI_VERSION 17
 
 /* status codes (negative: validation, nothing launched) */
 #define MSA_OK 0
@@ -388,6 +388,37 @@ int msa_decode_accumulate(const msa_tensor4* q, const msa_tensor4* k, const msa_
                           const msa_tensor4* o, const int32_t* lens, const msa_tensor4* scores_in,
                           const msa_tensor4* scores_out, float scale, void* workspace,
                           size_t workspace_bytes, msa_stream_t stream);
+
+/* Attention weights of the last S_q rows of a prompt, summed per key (no
+ * counterpart in the reference):
+ *   sums[b][g][j] (+)= sum over the heads h of kv head g and the rows i of
+ *                      softmax_i(q_bhi . k_bg * scale)[j]
+ * row i at position S_k - S_q + i, causal.  The scores msa_cache_evict takes.
+ *   q [B][H][S_q][D], k [B][H_kv][S_k][D], S_q <= S_k
+ *   sums: fp32 described as [B][H_kv][S_k][1], stride[2] = 1; add = 1 adds to
+ *         what it holds, 0 overwrites it
+ * Sums in a fixed order: the same call gives the same bits. */
+size_t msa_attention_weight_sums_workspace_bytes(const msa_tensor4* q, const msa_tensor4* k);
+int msa_attention_weight_sums(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* sums,
+                              int32_t add, float scale, void* workspace, size_t workspace_bytes,
+                              msa_stream_t stream);
+
+/* Eviction from a cache (no counterpart in the reference).  Of the n_b = lens[b]
+ * (clamped to [0, S]; NULL: S) keys of a sequence the first `sinks`, the last
+ * `recent` and the best scored others stay, `keep` in all, in their order; ties
+ * go to the lower position, a NaN score counts as the highest.  n_b <= keep: all
+ * stay.  Rows of the outputs behind the kept ones become 0, their positions -1.
+ *   k, v [B][H_kv][S][D] bf16, fp16 or fp32, D contiguous, any alignment
+ *   k_out, v_out [B][H_kv][keep][D], the same dtype, apart from k and v
+ *   scores, scores_out: fp32 described as [B][H_kv][S][1] and [B][H_kv][keep][1],
+ *         stride[2] = 1
+ *   positions [B][H_kv][keep] int32, contiguous; new_lens [B] int32
+ * 1 <= keep <= S, sinks >= 0, recent >= 0, sinks + recent <= keep. */
+int msa_cache_evict(const msa_tensor4* k, const msa_tensor4* v, const msa_tensor4* scores,
+                    const int32_t* lens, int64_t keep, int64_t recent, int64_t sinks,
+                    const msa_tensor4* k_out, const msa_tensor4* v_out,
+                    const msa_tensor4* scores_out, int32_t* positions, int32_t* new_lens,
+                    msa_stream_t stream);
 
 /* Rotary position embedding of one layer's query and key heads, one launch.
  * Replaces the apply_rotary_pos_emb call of the patched forward

@@ -1360,6 +1360,18 @@ int check_cache(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* v
   return MSA_OK;
 }
 
+// fp32 scores [B][H_kv][n][1] of the keys of k.
+int check_key_scores(const msa_tensor4* s, const msa_tensor4* k, int64_t n) {
+  if (s->size[0] != k->size[0] || s->size[1] != k->size[1] || s->size[2] != n || s->size[3] != 1)
+    return MSA_E_RANK;
+  if (s->dtype != MSA_DTYPE_FP32) return MSA_E_DTYPE;
+  if (n == 0) return MSA_OK;
+  if (!s->data) return MSA_E_NULL;
+  if ((n > 1 && s->stride[2] != 1) || (reinterpret_cast<uintptr_t>(s->data) & 3u) != 0)
+    return MSA_E_ALIGN;
+  return MSA_OK;
+}
+
 // q and o of the rows kernels.
 int check_rows_qo(const msa_tensor4* q, const msa_tensor4* o, float scale) {
   if (!q->data || !o->data) return MSA_E_NULL;
@@ -1455,16 +1467,9 @@ int msa_decode_accumulate(const msa_tensor4* q, const msa_tensor4* k, const msa_
   if (q->size[1] % k->size[1] != 0) return MSA_E_RANK;
   if (q->size[2] != 1) return MSA_E_SEQ;
   if (q->size[1] / k->size[1] > MSA_MAX_HEADS) return MSA_E_HEADS;
-  for (const msa_tensor4* s : {scores_in, scores_out}) {
-    if (s->size[0] != k->size[0] || s->size[1] != k->size[1] || s->size[2] != k->size[2] ||
-        s->size[3] != 1)
-      return MSA_E_RANK;
-    if (s->dtype != MSA_DTYPE_FP32) return MSA_E_DTYPE;
-    if (s->size[2] == 0) continue;
-    if (!s->data) return MSA_E_NULL;
-    if ((s->size[2] > 1 && s->stride[2] != 1) || (reinterpret_cast<uintptr_t>(s->data) & 3u) != 0)
-      return MSA_E_ALIGN;
-  }
+  st = check_key_scores(scores_in, k, k->size[2]);
+  if (st == MSA_OK) st = check_key_scores(scores_out, k, k->size[2]);
+  if (st != MSA_OK) return st;
   if (q->size[0] * k->size[1] > 65535) return MSA_E_HEADS;
   RowsParams rp;
   memset(&rp, 0, sizeof(rp));
@@ -1480,6 +1485,175 @@ int msa_decode_accumulate(const msa_tensor4* q, const msa_tensor4* k, const msa_
   rp.wo_sb = scores_out->stride[0]; rp.wo_sh = scores_out->stride[1];
   const hipError_t e = launch_rows(rp, true, q->dtype, o->dtype, int(q->size[3]),
                                    reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSA_OK : int(e);
+}
+
+// ---------------------------------------------------------------------------
+// attention weights summed per key; eviction
+// ---------------------------------------------------------------------------
+namespace {
+
+struct SumsLayout {
+  size_t stat_r, part, col_part, total;
+};
+
+int sums_plan(SumsParams& sp, SumsLayout& l, const msa_tensor4* q, const msa_tensor4* k) {
+  const int64_t B = q->size[0], H = q->size[1], Sq = q->size[2], D = q->size[3];
+  const int64_t Hkv = k->size[1], Sk = k->size[2], BH = B * H;
+  if (B > (1 << 24) || H > (1 << 24) || BH > (1 << 24) || BH * Sq > (int64_t(1) << 30) ||
+      BH * Sk > (int64_t(1) << 34))
+    return MSA_E_HEADS;
+  sp.batch = int(B);
+  sp.heads = int(H);
+  sp.kv_heads = int(Hkv);
+  sp.group = int(H / Hkv);
+  sp.s_q = int(Sq);
+  sp.s_k = int(Sk);
+  sp.s_q_pad = int(cdiv(Sq, 16) * 16);
+  const int tiles = sums_tiles(int(D));
+  sp.mt = Sq <= 16 ? 1 : tiles;
+  sp.n_rt = int(cdiv(Sq, 16 * sp.mt));
+  // stats: key splits where there are few row tiles
+  const int64_t items = BH * sp.n_rt;
+  const int64_t want = std::min<int64_t>(cdiv(Sk, 512), cdiv(1024, items));
+  sp.chunk = int(cdiv(cdiv(Sk, want), 128) * 128);
+  sp.n_split = items >= 512 ? 1 : int(cdiv(Sk, sp.chunk));
+  if (sp.n_split == 1) sp.chunk = int(cdiv(Sk, 128) * 128);
+  // columns: a key tile per wave where there are few rows for four waves; row
+  // splits where there are few key tiles
+  const int64_t blocks = sp.s_q_pad / 16 * sp.group;  // 16-row blocks of the first keys
+  sp.wave_keys = blocks < 64 && B * Hkv * cdiv(Sk, 64 * tiles) >= 512;
+  sp.n_kt = int(cdiv(Sk, 16 * tiles * (sp.wave_keys ? 4 : 1)));
+  const int64_t ci = B * Hkv * sp.n_kt;
+  sp.n_rsplit = ci >= 512 ? 1 : int(std::max<int64_t>(1, std::min(cdiv(1024, ci), blocks / 16)));
+  if (items * sp.n_split >= (int64_t(1) << 31) || ci * sp.n_rsplit >= (int64_t(1) << 31) ||
+      B * Hkv > 65535)
+    return MSA_E_HEADS;
+  const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t rows = size_t(BH) * sp.s_q_pad;
+  l.stat_r = up(rows * 4);
+  l.part = l.stat_r + up(rows * 4);
+  l.col_part = l.part + (sp.n_split > 1 ? up(rows * 8 * sp.n_split) : 0);
+  l.total = l.col_part + (sp.n_rsplit > 1 ? up(size_t(B) * Hkv * Sk * 4 * sp.n_rsplit) : 0);
+  return MSA_OK;
+}
+
+// D contiguous, strides not negative.
+bool evict_rows_ok(const msa_tensor4* t) {
+  if (t->size[3] > 1 && t->stride[3] != 1) return false;
+  if ((reinterpret_cast<uintptr_t>(t->data) % elem_size(t->dtype)) != 0) return false;
+  return t->stride[0] >= 0 && t->stride[1] >= 0 && t->stride[2] >= 0;
+}
+
+// Rows, base and strides of 16-byte units.
+bool evict_units16(const msa_tensor4* t) {
+  const int es = elem_size(t->dtype);
+  if ((reinterpret_cast<uintptr_t>(t->data) & 15u) != 0 || (t->size[3] * es & 15) != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t->size[i] > 1 && ((t->stride[i] * es) & 15) != 0) return false;
+  return true;
+}
+
+}  // namespace
+
+size_t msa_attention_weight_sums_workspace_bytes(const msa_tensor4* q, const msa_tensor4* k) {
+  if (!q || !k) return 0;
+  for (int i = 0; i < 4; ++i)
+    if (q->size[i] <= 0 || k->size[i] <= 0) return 0;
+  if (q->size[1] % k->size[1] != 0 || q->size[2] > k->size[2] || k->size[2] > kMaxSeq) return 0;
+  SumsParams sp;
+  SumsLayout l;
+  memset(&sp, 0, sizeof(sp));
+  return sums_plan(sp, l, q, k) == MSA_OK ? l.total : 0;
+}
+
+int msa_attention_weight_sums(const msa_tensor4* q, const msa_tensor4* k, const msa_tensor4* sums,
+                              int32_t add, float scale, void* workspace, size_t workspace_bytes,
+                              msa_stream_t stream) {
+  int st = check_qk(q, k);
+  if (st != MSA_OK) return st;
+  if (!sums) return MSA_E_NULL;
+  if (q->size[2] > k->size[2]) return MSA_E_SEQ;
+  st = check_key_scores(sums, k, k->size[2]);
+  if (st != MSA_OK) return st;
+  if (!(scale > 0.0f) || !isfinite(scale)) return MSA_E_HEADS;
+  if (add != 0 && add != 1) return MSA_E_FLAGS;
+  SumsParams sp;
+  SumsLayout l;
+  memset(&sp, 0, sizeof(sp));
+  st = sums_plan(sp, l, q, k);
+  if (st != MSA_OK) return st;
+  if (!workspace || workspace_bytes < l.total) return MSA_E_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return MSA_E_ALIGN;
+  sp.q = q->data; sp.k = k->data;
+  sp.q_sb = q->stride[0]; sp.q_sh = q->stride[1]; sp.q_ss = q->stride[2];
+  sp.k_sb = k->stride[0]; sp.k_sh = k->stride[1]; sp.k_ss = k->stride[2];
+  sp.sums = static_cast<float*>(sums->data);
+  sp.s_sb = sums->stride[0]; sp.s_sh = sums->stride[1];
+  sp.add = add;
+  sp.scale_log2 = float(double(scale) * 1.4426950408889634);
+  sp.stat_m = ws_at<float>(workspace, 0);
+  sp.stat_r = ws_at<float>(workspace, l.stat_r);
+  sp.part = ws_at<float>(workspace, l.part);
+  sp.col_part = ws_at<float>(workspace, l.col_part);
+  const hipError_t e = launch_sums(sp, q->dtype, int(q->size[3]), reinterpret_cast<hipStream_t>(stream));
+  return e == hipSuccess ? MSA_OK : int(e);
+}
+
+int msa_cache_evict(const msa_tensor4* k, const msa_tensor4* v, const msa_tensor4* scores,
+                    const int32_t* lens, int64_t keep, int64_t recent, int64_t sinks,
+                    const msa_tensor4* k_out, const msa_tensor4* v_out,
+                    const msa_tensor4* scores_out, int32_t* positions, int32_t* new_lens,
+                    msa_stream_t stream) {
+  if (!k || !v || !scores || !k_out || !v_out || !scores_out || !positions || !new_lens)
+    return MSA_E_NULL;
+  const msa_tensor4* ts[4] = {k, v, k_out, v_out};
+  for (const msa_tensor4* t : ts) {
+    if (!t->data) return MSA_E_NULL;
+    for (int i = 0; i < 4; ++i)
+      if (t->size[i] <= 0 || (i != 2 && t->size[i] != k->size[i])) return MSA_E_RANK;
+    if (t->dtype != k->dtype || elem_size(t->dtype) == 0) return MSA_E_DTYPE;
+  }
+  if (v->size[2] != k->size[2] || k_out->size[2] != keep || v_out->size[2] != keep)
+    return MSA_E_RANK;
+  if (k->size[2] > kMaxSeq) return MSA_E_SEQ;
+  if (keep < 1 || keep > k->size[2] || recent < 0 || sinks < 0 || sinks > keep ||
+      recent > keep - sinks)
+    return MSA_E_TOPK;
+  int st = check_key_scores(scores, k, k->size[2]);
+  if (st == MSA_OK) st = check_key_scores(scores_out, k, keep);
+  if (st != MSA_OK) return st;
+  for (const msa_tensor4* t : ts)
+    if (!evict_rows_ok(t)) return MSA_E_ALIGN;
+  if (k->size[0] > 65535 || k->size[1] > 65535 || k->size[0] * k->size[1] > 65535 ||
+      k->size[3] > 65536)
+    return MSA_E_HEADS;
+  EvictParams ep;
+  memset(&ep, 0, sizeof(ep));
+  const int es = elem_size(k->dtype);
+  ep.k = k->data; ep.v = v->data; ep.ko = k_out->data; ep.vo = v_out->data;
+  ep.scores = static_cast<const float*>(scores->data);
+  ep.scores_out = static_cast<float*>(scores_out->data);
+  ep.lens = lens;
+  ep.pos = positions;
+  ep.new_lens = new_lens;
+  ep.k_sb = k->stride[0] * es; ep.k_sh = k->stride[1] * es; ep.k_ss = k->stride[2] * es;
+  ep.v_sb = v->stride[0] * es; ep.v_sh = v->stride[1] * es; ep.v_ss = v->stride[2] * es;
+  ep.ko_sb = k_out->stride[0] * es; ep.ko_sh = k_out->stride[1] * es; ep.ko_ss = k_out->stride[2] * es;
+  ep.vo_sb = v_out->stride[0] * es; ep.vo_sh = v_out->stride[1] * es; ep.vo_ss = v_out->stride[2] * es;
+  ep.s_sb = scores->stride[0]; ep.s_sh = scores->stride[1];
+  ep.so_sb = scores_out->stride[0]; ep.so_sh = scores_out->stride[1];
+  ep.batch = int(k->size[0]);
+  ep.kv_heads = int(k->size[1]);
+  ep.s = int(k->size[2]);
+  ep.keep = int(keep);
+  ep.recent = int(recent);
+  ep.sinks = int(sinks);
+  ep.unit = 16;
+  for (const msa_tensor4* t : ts)
+    if (!evict_units16(t)) ep.unit = 2;
+  ep.upr = int(k->size[3] * es / ep.unit);
+  const hipError_t e = launch_evict(ep, reinterpret_cast<hipStream_t>(stream));
   return e == hipSuccess ? MSA_OK : int(e);
 }
 

@@ -253,6 +253,42 @@ struct RowsParams {
 };
 constexpr int kRowsMaxSplit = 2048;  // splits of one row, prefix and own together
 
+// Attention weights summed per key (sums_*_kernel).
+struct SumsParams {
+  const void* q;  // [batch][heads][s_q][D]: rows s_k - s_q .. s_k - 1
+  const void* k;  // [batch][kv_heads][s_k][D]
+  int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss;
+  float* sums;    // [batch][kv_heads][s_k]
+  int64_t s_sb, s_sh;
+  int add;        // 1: added to what is there
+  int batch, heads, kv_heads, group, s_q, s_k, s_q_pad;  // s_q_pad: s_q to 16
+  float scale_log2;
+  int mt, n_rt, n_split, chunk;   // stats: row tiles of an item, items, key splits
+  int n_kt, n_rsplit, wave_keys;  // columns: key tiles, row splits; 1: a key tile per wave
+  float* part;      // n_split > 1: (m, l) [n_split][batch * heads][s_q_pad]
+  float* stat_m;    // [batch * heads][s_q_pad]: max of the row's scores, log2 units
+  float* stat_r;    // 1 / sum
+  float* col_part;  // n_rsplit > 1: [n_rsplit][batch * kv_heads][s_k]
+};
+
+// Eviction (evict_*_kernel).  Strides of k, v, ko and vo in bytes.
+struct EvictParams {
+  const void* k;  // [batch][kv_heads][s] rows
+  const void* v;
+  void* ko;       // [batch][kv_heads][keep] rows
+  void* vo;
+  const float* scores;  // [batch][kv_heads][s]
+  float* scores_out;    // [batch][kv_heads][keep]
+  const int32_t* lens;  // [batch] or nullptr: s
+  int32_t* pos;         // [batch][kv_heads][keep], contiguous
+  int32_t* new_lens;    // [batch]
+  int64_t k_sb, k_sh, k_ss, v_sb, v_sh, v_ss;
+  int64_t ko_sb, ko_sh, ko_ss, vo_sb, vo_sh, vo_ss;
+  int64_t s_sb, s_sh, so_sb, so_sh;
+  int batch, kv_heads, s, keep, recent, sinks;
+  int unit, upr;  // bytes of a copied unit (16 or 2), units of a row
+};
+
 // Rotary embedding of one layer's q and k heads (rope_kernel).  q/k/qo/ko
 // strides are [B][H][S][D] element strides; cos/sin are [B or 1][S][rot]
 // (c_sb / n_sb = 0 broadcasts one table over the batch).  n_pair = rot / 16
@@ -322,6 +358,9 @@ hipError_t launch_vs_estimate(const VsEstParams& p, int dtype, int D, hipStream_
 hipError_t launch_block_lists(const ListParams& p, hipStream_t st);
 hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,
                        hipStream_t st);
+int sums_tiles(int D);  // 16-row (16-key) tiles of a stats (columns) item
+hipError_t launch_sums(const SumsParams& p, int dtype, int D, hipStream_t st);
+hipError_t launch_evict(const EvictParams& p, hipStream_t st);
 hipError_t launch_round(const RoundParams& p, int n, hipStream_t st);
 hipError_t launch_rope(const RopeParams& p, int dtype, hipStream_t st);
 

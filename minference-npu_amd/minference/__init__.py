@@ -3,7 +3,8 @@
 Same public names as the reference package (MInference-NPU/minference/__init__.py:8-44):
 MInference, MInferenceConfig, minference_patch, patch_hf, get_support_models,
 block_sparse_attention, streaming_forward; plus dense_attention and the cache
-operators (shared_prefix_attention, decode_accumulate).
+operators (shared_prefix_attention, decode_accumulate, attention_weight_sums,
+evict_kv_cache).
 """
 
 from .configs.model2path import get_support_models
@@ -20,6 +21,8 @@ __all__ = [
     "dense_attention",
     "shared_prefix_attention",
     "decode_accumulate",
+    "attention_weight_sums",
+    "evict_kv_cache",
 ]
 
 
@@ -56,4 +59,8 @@ def __getattr__(name):
         from .backend import cached
 
         return getattr(cached, name)
+    if name in ("attention_weight_sums", "evict_kv_cache"):
+        from .ops import kv_eviction
+
+        return getattr(kv_eviction, name)
     raise AttributeError(name)

@@ -55,7 +55,7 @@ MSA_ESTIMATE_SELECT_ONLY = 8
 
 MSA_MAX_HEADS = 128
 MSA_BLOCK = 64
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 _DTYPE_CODE = {
     torch.bfloat16: MSA_DTYPE_BF16,
@@ -91,6 +91,9 @@ EXPORTED_SYMBOLS = (
     "msa_shared_prefix_attention",
     "msa_decode_accumulate_workspace_bytes",
     "msa_decode_accumulate",
+    "msa_attention_weight_sums_workspace_bytes",
+    "msa_attention_weight_sums",
+    "msa_cache_evict",
 )
 
 
@@ -295,6 +298,17 @@ def load_library() -> ctypes.CDLL:
         lib.msa_decode_accumulate.argtypes = [T4] * 4 + [ctypes.c_void_p, T4, T4] + [
             ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
         ]
+        lib.msa_attention_weight_sums_workspace_bytes.restype = ctypes.c_size_t
+        lib.msa_attention_weight_sums_workspace_bytes.argtypes = [T4] * 2
+        lib.msa_attention_weight_sums.restype = ctypes.c_int
+        lib.msa_attention_weight_sums.argtypes = [T4] * 3 + [
+            ctypes.c_int32, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
+        ]
+        lib.msa_cache_evict.restype = ctypes.c_int
+        lib.msa_cache_evict.argtypes = [T4] * 3 + [
+            ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, T4, T4, T4,
+            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+        ]
         ver = lib.msa_abi_version()
         if ver != ABI_VERSION:
             raise ImportError(f"libmsa ABI version {ver} != expected {ABI_VERSION}")
@@ -385,7 +399,7 @@ def _lens_ptr(lens: Optional[torch.Tensor], batch: int, device: torch.device) ->
         return None
     if (lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous()
             or lens.device != device):
-        raise ValueError(f"lens must be a contiguous int32 [{batch}] tensor on q's device, got "
+        raise ValueError(f"lens must be a contiguous int32 [{batch}] tensor on the caches' device, got "
                          f"{tuple(lens.shape)} {lens.dtype} on {lens.device}")
     return lens.data_ptr()
 
@@ -419,6 +433,32 @@ def decode_accumulate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: to
         check(lib.msa_decode_accumulate(qd, kd, vd, od, lens_p, sd, rd, float(scale),
                                         ws.data_ptr(), ws.numel(),
                                         current_stream_handle(q.device)))
+
+
+def attention_weight_sums(q: torch.Tensor, k: torch.Tensor, sums: torch.Tensor, add: bool,
+                          scale: float) -> None:
+    """Launch msa_attention_weight_sums on the current stream of q's device:
+    sums fp32 [B,H_kv,S_k], added to when ``add``."""
+    lib = load_library()
+    qd, kd, sd = (ctypes.byref(tensor4(t)) for t in (q, k, sums.unsqueeze(-1)))
+    with torch.cuda.device(q.device):
+        ws = workspace(lib.msa_attention_weight_sums_workspace_bytes(qd, kd), q.device)
+        check(lib.msa_attention_weight_sums(qd, kd, sd, int(add), float(scale), ws.data_ptr(),
+                                            ws.numel(), current_stream_handle(q.device)))
+
+
+def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
+                lens: Optional[torch.Tensor], keep: int, recent: int, sinks: int,
+                k_out: torch.Tensor, v_out: torch.Tensor, scores_out: torch.Tensor,
+                positions: torch.Tensor, new_lens: torch.Tensor) -> None:
+    """Launch msa_cache_evict on the current stream of k's device."""
+    lens_p = _lens_ptr(lens, k.shape[0], k.device)
+    kd, vd, sd, kod, vod, sod = (ctypes.byref(tensor4(t)) for t in (
+        k, v, scores.unsqueeze(-1), k_out, v_out, scores_out.unsqueeze(-1)))
+    with torch.cuda.device(k.device):
+        check(load_library().msa_cache_evict(
+            kd, vd, sd, lens_p, keep, recent, sinks, kod, vod, sod, positions.data_ptr(),
+            new_lens.data_ptr(), current_stream_handle(k.device)))
 
 
 def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

@@ -17,6 +17,7 @@ import torch
 from .. import _abi
 from ..ops.common import (SUPPORTED_DTYPES, accepts_float32, check_written, dense_scale,
                           kernel_head_dim, kernel_view, make_out, pad_head_dim)
+from ..ops.kv_eviction import check_scores
 
 __all__ = ["shared_prefix_attention", "decode_accumulate"]
 
@@ -105,16 +106,6 @@ def shared_prefix_attention(
     return result
 
 
-def _check_scores(name: str, t: torch.Tensor, k_cache: torch.Tensor) -> None:
-    if tuple(t.shape) != tuple(k_cache.shape[:3]) or t.dtype != torch.float32:
-        raise ValueError(f"{name} must be float32 {tuple(k_cache.shape[:3])}, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    if t.device != k_cache.device:
-        raise ValueError(f"{name} must be on the cache's device")
-    if t.shape[2] > 1 and t.stride(2) != 1:
-        raise ValueError(f"{name} must be contiguous over the keys")
-
-
 @accepts_float32(("q", "k_cache", "v_cache"), once=True)
 def decode_accumulate(
     q: torch.Tensor,
@@ -147,11 +138,11 @@ def decode_accumulate(
     _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
     if q.shape[2] != 1:
         raise NotImplementedError("decode_accumulate takes one query row")
-    _check_scores("scores", scores, k_cache)
+    check_scores("scores", scores, k_cache.shape[:3], k_cache.device)
     if scores_out is None:
         scores_out = scores
     else:
-        _check_scores("scores_out", scores_out, k_cache)
+        check_scores("scores_out", scores_out, k_cache.shape[:3], k_cache.device)
     same = scores_out.data_ptr() == scores.data_ptr() and scores_out.stride() == scores.stride()
     check_written("scores_out", scores_out, () if same else (("scores", scores),))
     s = dense_scale(q.shape[-1]) if scale is None else float(scale)

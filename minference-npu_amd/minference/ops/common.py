@@ -250,10 +250,44 @@ def make_out(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
     return out
 
 
-def _span(t: torch.Tensor):
-    """First and last byte of t's elements (t not empty)."""
-    a = t.data_ptr()
-    return a, a + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) - 1
+def _may_meet(diff: int, dims) -> bool:
+    """Whether diff = sum of x_i * stride_i for some lo_i <= x_i <= hi_i, dims =
+    [(stride, lo, hi)] from the largest stride down (each larger than what the
+    ones behind it span)."""
+    if not dims:
+        return diff == 0
+    st, lo, hi = dims[0]
+    q = diff // st
+    return any(lo <= x <= hi and _may_meet(diff - x * st, dims[1:]) for x in (q, q + 1))
+
+
+def _share(t: torch.Tensor, u: torch.Tensor) -> bool:
+    """Whether an element of t lies where one of u does.  Views of one layout (k
+    and v side by side in one buffer) are told apart exactly; of others, whose
+    extents overlap, sharing is assumed."""
+    def end(x):
+        return x.data_ptr() + x.element_size() * (
+            1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+
+    if t.data_ptr() >= end(u) or u.data_ptr() >= end(t):
+        return False
+    diff, es = u.data_ptr() - t.data_ptr(), t.element_size()
+    if t.dim() != u.dim() or es != u.element_size() or diff % es:
+        return True
+    dims = []
+    for n, s, m, r in zip(t.shape, t.stride(), u.shape, u.stride()):
+        if n == 1 and m == 1:
+            continue
+        if n > 1 and m > 1 and s != r or (s if n > 1 else r) == 0:
+            return True
+        dims.append((s if n > 1 else r, 1 - m, n - 1))
+    dims.sort(reverse=True)
+    span = 0
+    for st, lo, hi in reversed(dims):
+        if st <= span:
+            return True
+        span += st * max(-lo, hi)
+    return _may_meet(diff // es, dims)
 
 
 def check_written(name: str, t: torch.Tensor, others=()) -> None:
@@ -261,18 +295,14 @@ def check_written(name: str, t: torch.Tensor, others=()) -> None:
     (name, tensor) ``others``."""
     if t.numel() == 0:
         return
-    inner = 1
+    span = 0
     for st, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
-        if st < inner:
+        if st <= span:
             raise ValueError(f"{name} has elements that share memory (shape {tuple(t.shape)}, "
                              f"strides {t.stride()})")
-        inner = st * (n - 1) + inner
-    lo, hi = _span(t)
+        span += st * (n - 1)
     for other, u in others:
-        if u.numel() == 0:
-            continue
-        ulo, uhi = _span(u)
-        if lo <= uhi and ulo <= hi:
+        if u.numel() and _share(t, u):
             raise ValueError(f"{name} shares memory with {other}")
 
 

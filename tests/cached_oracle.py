@@ -73,3 +73,24 @@ def decode_accumulate(q, k, v, scores, lens, scale):
         out[b] = o
         upd[b, :, :n] += p[:, 0].reshape(Hkv, group, n).sum(1)
     return out, upd
+
+
+def weight_sums(q, k, scale):
+    """[B, H_kv, S_k] in 64 bits: causal softmax weights summed over rows and heads."""
+    B, H, Sq, _ = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    see = torch.arange(Sk) <= torch.arange(Sq)[:, None] + (Sk - Sq)
+    kk = repeat_kv(k, H // Hkv).double()
+    _, p = attention(q.double(), kk, kk, see, scale)
+    p = torch.where(see, p, torch.zeros((), dtype=p.dtype))
+    return p.sum(2).reshape(B, Hkv, H // Hkv, Sk).sum(2)
+
+
+def kept_positions(scores, n, keep, recent, sinks):
+    """Positions one kv head keeps, ascending: scores [S] (NaN highest, ties low)."""
+    if n <= keep:
+        return list(range(n))
+    sure = set(range(sinks)) | set(range(n - recent, n))
+    free = [j for j in range(n) if j not in sure]
+    free.sort(key=lambda j: (0, 0.0, j) if scores[j] != scores[j] else (1, -scores[j], j))
+    return sorted(sure | set(free[:keep - len(sure)]))
