@@ -87,12 +87,14 @@ __global__ __launch_bounds__(256) void sums_stats_kernel(const SumsParams P) {
             u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, koff + 16u * u * kss + 64 * ks, 0, 0));
   };
 
-  float m[MT], mp[MT], l[MT];  // of the keys this lane sees
+  // of the keys this lane sees: running max, what the exponentials are taken
+  // against, and the sum in two levels (small terms are not lost in a long sum)
+  float m[MT], mp[MT], l[MT], part[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     m[mt] = -__builtin_inff();
     mp[mt] = 0.0f;
-    l[mt] = 0.0f;
+    l[mt] = part[mt] = 0.0f;
   }
   const float c = P.scale_log2;
   auto block = [&](int j0, const u32x4 (&kr)[2][NKS]) INLINE {
@@ -119,14 +121,23 @@ __global__ __launch_bounds__(256) void sums_stats_kernel(const SumsParams P) {
       if (__ballot(bm > m[mt] + 16.0f) != 0) {
         const float mn = fmaxf(m[mt], bm);
         mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
-        l[mt] *= __builtin_amdgcn_exp2f(m[mt] - mp[mt]);
+        const float al = __builtin_amdgcn_exp2f(m[mt] - mp[mt]);
+        l[mt] *= al;
+        part[mt] *= al;
         m[mt] = mn;
       }
+      float e[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int j = 0; j < 8; ++j)
+        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], c, -mp[mt]));
+      part[mt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+    }
+  };
+  auto flush = [&]() INLINE {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          l[mt] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][i], c, -mp[mt]));
+    for (int mt = 0; mt < MT; ++mt) {
+      l[mt] += part[mt];
+      part[mt] = 0.0f;
     }
   };
   const int first = j_begin + KB * w;
@@ -141,7 +152,9 @@ __global__ __launch_bounds__(256) void sums_stats_kernel(const SumsParams P) {
       if (i + 1 >= nblk) break;
       load_block(jb(i + 2), ka);
       block(jb(i + 1), kb);
+      if ((i & 14) == 14) flush();
     }
+    flush();
   }
 
   // merge a row's lanes, then the waves

@@ -58,9 +58,11 @@ def __getattr__(name):
     if name in ("shared_prefix_attention", "decode_accumulate"):
         from .backend import cached
 
-        return getattr(cached, name)
+        globals()[name] = getattr(cached, name)
+        return globals()[name]
     if name in ("attention_weight_sums", "evict_kv_cache"):
         from .ops import kv_eviction
 
-        return getattr(kv_eviction, name)
+        globals()[name] = getattr(kv_eviction, name)
+        return globals()[name]
     raise AttributeError(name)

@@ -285,7 +285,7 @@ def load_library() -> ctypes.CDLL:
             ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32,
             ctypes.c_void_p,
         ]
-        T4 = ctypes.POINTER(MsaTensor4)
+        T4 = ctypes.c_void_p  # address of an MsaTensor4
         lib.msa_shared_prefix_workspace_bytes.restype = ctypes.c_size_t
         lib.msa_shared_prefix_workspace_bytes.argtypes = [T4] * 5
         lib.msa_shared_prefix_attention.restype = ctypes.c_int
@@ -404,6 +404,43 @@ def _lens_ptr(lens: Optional[torch.Tensor], batch: int, device: torch.device) ->
     return lens.data_ptr()
 
 
+_MAX_DESCS = 8
+_DESC_PACK = [struct.Struct("@" + "P4q4qii" * n) for n in range(_MAX_DESCS + 1)]
+_DESCS = threading.local()
+
+
+def _descriptors(tensors: Sequence[torch.Tensor]) -> list:
+    """Addresses of descriptors of [B,H,S,D] tensors, or of [B,H,S] ones as
+    [B,H,S,1], in one pack into a buffer of this thread that the next call
+    overwrites (six tensors: 4 us, 11 as tensor4 each)."""
+    buf = getattr(_DESCS, "buf", None)
+    if buf is None:
+        buf = _DESCS.buf = ctypes.create_string_buffer(_TENSOR4.size * _MAX_DESCS)
+        _DESCS.at = [ctypes.addressof(buf) + _TENSOR4.size * i for i in range(_MAX_DESCS)]
+    vals = []
+    for t in tensors:
+        code = _DTYPE_CODE.get(t.dtype)
+        if code is None:
+            raise TypeError(f"unsupported dtype {t.dtype}")
+        if t.dim() == 4:
+            vals += (t.data_ptr(), *t.shape, *t.stride(), code, 0)
+        elif t.dim() == 3:
+            vals += (t.data_ptr(), *t.shape, 1, *t.stride(), 1, code, 0)
+        else:
+            raise ValueError(f"expected a [B,H,S,D] or [B,H,S] tensor, got {t.dim()}-D")
+    _DESC_PACK[len(tensors)].pack_into(buf, 0, *vals)
+    return _DESCS.at
+
+
+def _on_device(device: torch.device, fn) -> None:
+    """fn(stream handle) with ``device`` current, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        fn(current_stream_handle(device))
+        return
+    with torch.cuda.device(device):
+        fn(current_stream_handle(device))
+
+
 def shared_prefix_attention(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, k: torch.Tensor,
                             v: torch.Tensor, out: torch.Tensor, lens: Optional[torch.Tensor],
                             scale: float) -> None:
@@ -412,11 +449,14 @@ def shared_prefix_attention(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor,
     k/v [B,H_kv,S_c,D]."""
     lib = load_library()
     lens_p = _lens_ptr(lens, q.shape[0], q.device)
-    ds = [ctypes.byref(tensor4(t)) for t in (q, kp, vp, k, v, out)]
-    with torch.cuda.device(q.device):
-        ws = workspace(lib.msa_shared_prefix_workspace_bytes(*ds[:5]), q.device)
-        check(lib.msa_shared_prefix_attention(*ds, lens_p, float(scale), ws.data_ptr(), ws.numel(),
-                                              current_stream_handle(q.device)))
+    d = _descriptors((q, kp, vp, k, v, out))
+
+    def launch(stream):
+        ws = workspace(lib.msa_shared_prefix_workspace_bytes(d[0], d[1], d[2], d[3], d[4]), q.device)
+        check(lib.msa_shared_prefix_attention(d[0], d[1], d[2], d[3], d[4], d[5], lens_p, scale,
+                                              ws.data_ptr(), ws.numel(), stream))
+
+    _on_device(q.device, launch)
 
 
 def decode_accumulate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -426,13 +466,14 @@ def decode_accumulate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: to
     [B,H,1,D] against the cache k/v; scores and scores_out fp32 [B,H_kv,S]."""
     lib = load_library()
     lens_p = _lens_ptr(lens, q.shape[0], q.device)
-    qd, kd, vd, od, sd, rd = (ctypes.byref(tensor4(t)) for t in (
-        q, k, v, out, scores.unsqueeze(-1), scores_out.unsqueeze(-1)))
-    with torch.cuda.device(q.device):
-        ws = workspace(lib.msa_decode_accumulate_workspace_bytes(qd, kd, vd), q.device)
-        check(lib.msa_decode_accumulate(qd, kd, vd, od, lens_p, sd, rd, float(scale),
-                                        ws.data_ptr(), ws.numel(),
-                                        current_stream_handle(q.device)))
+    d = _descriptors((q, k, v, out, scores, scores_out))
+
+    def launch(stream):
+        ws = workspace(lib.msa_decode_accumulate_workspace_bytes(d[0], d[1], d[2]), q.device)
+        check(lib.msa_decode_accumulate(d[0], d[1], d[2], d[3], lens_p, d[4], d[5], scale,
+                                        ws.data_ptr(), ws.numel(), stream))
+
+    _on_device(q.device, launch)
 
 
 def attention_weight_sums(q: torch.Tensor, k: torch.Tensor, sums: torch.Tensor, add: bool,
@@ -440,11 +481,14 @@ def attention_weight_sums(q: torch.Tensor, k: torch.Tensor, sums: torch.Tensor, 
     """Launch msa_attention_weight_sums on the current stream of q's device:
     sums fp32 [B,H_kv,S_k], added to when ``add``."""
     lib = load_library()
-    qd, kd, sd = (ctypes.byref(tensor4(t)) for t in (q, k, sums.unsqueeze(-1)))
-    with torch.cuda.device(q.device):
-        ws = workspace(lib.msa_attention_weight_sums_workspace_bytes(qd, kd), q.device)
-        check(lib.msa_attention_weight_sums(qd, kd, sd, int(add), float(scale), ws.data_ptr(),
-                                            ws.numel(), current_stream_handle(q.device)))
+    d = _descriptors((q, k, sums))
+
+    def launch(stream):
+        ws = workspace(lib.msa_attention_weight_sums_workspace_bytes(d[0], d[1]), q.device)
+        check(lib.msa_attention_weight_sums(d[0], d[1], d[2], int(add), scale, ws.data_ptr(),
+                                            ws.numel(), stream))
+
+    _on_device(q.device, launch)
 
 
 def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
@@ -452,13 +496,12 @@ def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
                 k_out: torch.Tensor, v_out: torch.Tensor, scores_out: torch.Tensor,
                 positions: torch.Tensor, new_lens: torch.Tensor) -> None:
     """Launch msa_cache_evict on the current stream of k's device."""
+    lib = load_library()
     lens_p = _lens_ptr(lens, k.shape[0], k.device)
-    kd, vd, sd, kod, vod, sod = (ctypes.byref(tensor4(t)) for t in (
-        k, v, scores.unsqueeze(-1), k_out, v_out, scores_out.unsqueeze(-1)))
-    with torch.cuda.device(k.device):
-        check(load_library().msa_cache_evict(
-            kd, vd, sd, lens_p, keep, recent, sinks, kod, vod, sod, positions.data_ptr(),
-            new_lens.data_ptr(), current_stream_handle(k.device)))
+    d = _descriptors((k, v, scores, k_out, v_out, scores_out))
+    _on_device(k.device, lambda stream: check(lib.msa_cache_evict(
+        d[0], d[1], d[2], lens_p, keep, recent, sinks, d[3], d[4], d[5], positions.data_ptr(),
+        new_lens.data_ptr(), stream)))
 
 
 def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

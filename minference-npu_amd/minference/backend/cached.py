@@ -24,28 +24,30 @@ __all__ = ["shared_prefix_attention", "decode_accumulate"]
 
 def _check_caches(q: torch.Tensor, pairs) -> None:
     """Shapes, types and devices of (name, k, v, batch) cache pairs against q."""
-    if q.dim() != 4:
-        raise ValueError(f"q must be 4-D [B,H,S,D], got {q.dim()}-D")
-    tensors = [q]
+    qs = q.shape
+    if len(qs) != 4:
+        raise ValueError(f"q must be 4-D [B,H,S,D], got {len(qs)}-D")
+    kv_heads = pairs[0][1].shape[1] if pairs[0][1].dim() > 1 else 0
     for name, k, v, batch in pairs:
-        if k.dim() != 4 or v.shape != k.shape:
+        ks = k.shape
+        if len(ks) != 4 or v.shape != ks:
             raise ValueError(f"k and v of the {name} must be 4-D [B,H_kv,S,D] of one shape, got "
-                             f"{tuple(k.shape)} and {tuple(v.shape)}")
-        if k.shape[0] != batch or k.shape[3] != q.shape[3]:
-            raise ValueError(f"the {name} must be [{batch},H_kv,S,{q.shape[3]}] for q "
-                             f"{tuple(q.shape)}, got {tuple(k.shape)}")
-        if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
-            raise ValueError(f"q heads {q.shape[1]} not a multiple of {name} heads {k.shape[1]}")
-        tensors += [k, v]
-    if len({p[1].shape[1] for p in pairs}) != 1:
-        raise ValueError("prefix and own caches must have the same kv heads")
-    _abi.require_device(*tensors)
-    for t in tensors:
-        if t.dtype not in SUPPORTED_DTYPES:
-            raise NotImplementedError(f"the MI355X kernels take bf16 or fp16 inputs, got {t.dtype}")
-        if t.dtype != q.dtype:
+                             f"{tuple(ks)} and {tuple(v.shape)}")
+        if ks[0] != batch or ks[3] != qs[3]:
+            raise ValueError(f"the {name} must be [{batch},H_kv,S,{qs[3]}] for q {tuple(qs)}, got "
+                             f"{tuple(ks)}")
+        if ks[1] < 1 or qs[1] % ks[1]:
+            raise ValueError(f"q heads {qs[1]} not a multiple of {name} heads {ks[1]}")
+        if ks[1] != kv_heads:
+            raise ValueError("prefix and own caches must have the same kv heads")
+    _abi.require_device(q, *(t for p in pairs for t in p[1:3]))
+    dt = q.dtype
+    if dt not in SUPPORTED_DTYPES:
+        raise NotImplementedError(f"the MI355X kernels take bf16 or fp16 inputs, got {dt}")
+    for _, k, v, _ in pairs:
+        if k.dtype != dt or v.dtype != dt:
             raise ValueError("q, k and v must share one dtype")
-    if q.shape[3] < 1:
+    if qs[3] < 1:
         raise ValueError("head_dim must be positive")
 
 
