@@ -1317,13 +1317,12 @@ int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const
   rp.mt = D > 128 || R <= 16 ? 1 : R <= 32 ? 2 : 4;
   rp.n_rt = int(cdiv(R, 16 * rp.mt));
   rp.n_rto = int(cdiv(rows, 16));
-  const int64_t slots = 512;
-  rows_split(Sp, std::min<int64_t>(cdiv(Sp, 256), cdiv(slots, rp.n_rt * Hkv)),
+  rows_split(Sp, std::min<int64_t>(cdiv(Sp, 256), cdiv(512, rp.n_rt * Hkv)),
              kp ? rows_max_chunk(kp, vp) : 128, rp.n_sp, rp.chunk_p);
-  rows_split(Sc, std::min<int64_t>(cdiv(Sc, 256), cdiv(slots, rp.n_rto * B * Hkv)),
+  rows_split(Sc, std::min<int64_t>(cdiv(Sc, 256), cdiv(2048, rp.n_rto * B * Hkv)),
              rows_max_chunk(k, v), rp.n_so, rp.chunk_o);
   if (rp.n_sp + rp.n_so > kRowsMaxSplit) return MSA_E_SEQ;
-  const int64_t np = Hkv * rp.n_sp * rp.n_rt, no = B * Hkv * rp.n_so * rp.n_rto;
+  const int64_t np = cdiv(Hkv * rp.n_sp, 8) * 8 * rp.n_rt, no = B * Hkv * rp.n_so * rp.n_rto;
   if (np + no >= (int64_t(1) << 31)) return MSA_E_HEADS;
   rp.n_prefix_items = int(np);
   rp.n_items = int(np + no);

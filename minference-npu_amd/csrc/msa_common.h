@@ -85,6 +85,16 @@ __device__ inline f32x4 mfma_qk<F16>(u32x4 a, u32x4 b, f32x4 c) {
                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Largest of eight scores, NaN if one is (a NaN score makes its row NaN
+// whatever the maximum is): four three-way maxima, where fmaxf would first
+// quiet each operand.
+__device__ inline float max8(f32x4 a, f32x4 b) {
+  const float x = __builtin_elementwise_maximum(__builtin_elementwise_maximum(a[0], a[1]), a[2]);
+  const float y = __builtin_elementwise_maximum(__builtin_elementwise_maximum(a[3], b[0]), b[1]);
+  const float z = __builtin_elementwise_maximum(__builtin_elementwise_maximum(b[2], b[3]), x);
+  return __builtin_elementwise_maximum(y, z);
+}
+
 __device__ inline u32x4 load16(const void* p) {
   return *reinterpret_cast<const u32x4*>(p);
 }

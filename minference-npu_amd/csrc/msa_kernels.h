@@ -240,7 +240,7 @@ struct RowsParams {
   int mt;                    // 16-row tiles of a prefix item
   int n_rt, n_sp, chunk_p;   // prefix: row tiles, key splits, keys of a split
   int n_rto, n_so, chunk_o;  // own caches: the same per (sequence, kv head)
-  int n_prefix_items, n_items;
+  int n_prefix_items, n_items;  // prefix: (kv head, split) pairs to a multiple of 8
   float scale_log2;          // softmax scale * log2(e)
   float* part;               // partial O, [row][D]: prefix [kv_heads][n_sp][batch * rows],
                              // from own_row0 on own [batch][kv_heads][n_so][rows]

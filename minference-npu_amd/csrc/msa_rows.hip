@@ -23,7 +23,8 @@
 //     P already lies.  V (A operand) is loaded by rows, a lane holding E = D /
 //     16 (8 from D = 128 on) dims of its 8 keys, and pairs of keys are put
 //     together by byte permutes; MFMA e takes dim E lc + e of every lane.
-// No LDS in the loop, and K and V are read once per item.  Softmax statistics
+// K goes through LDS (each wave its own block, no barrier), V straight from its
+// rows; both are read once per item.  Softmax statistics
 // and O are fp32; a row's running max moves only when a block exceeds it by
 // 2^kSlack.  P is rounded to the inputs' type twice, P and what that rounding
 // left, so the product's error stays below the output's own rounding.
@@ -32,6 +33,7 @@
 
 #include "msa_common.h"
 #include "msa_kernels.h"
+#include "msa_tile.h"
 
 namespace msa {
 
@@ -66,19 +68,19 @@ __device__ inline bool any_nonfinite(uint32_t x) {
   return (x & e) == e || (x & (e << 16)) == (e << 16);
 }
 
-template <int W>
+template <int W, int AUX>
 __device__ inline void load_words(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t soff,
                                   uint32_t (&w)[W]) {
   if constexpr (W == 4) {
-    const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, soff, 2));
+    const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, soff, AUX));
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = x[i];
   } else if constexpr (W == 3) {
-    const u32x3 x = __builtin_bit_cast(u32x3, __builtin_amdgcn_raw_buffer_load_b96(rs, off, soff, 2));
+    const u32x3 x = __builtin_bit_cast(u32x3, __builtin_amdgcn_raw_buffer_load_b96(rs, off, soff, AUX));
 #pragma unroll
     for (int i = 0; i < 3; ++i) w[i] = x[i];
   } else {
-    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off, soff, 2));
+    const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, off, soff, AUX));
 #pragma unroll
     for (int i = 0; i < 2; ++i) w[i] = x[i];
   }
@@ -106,9 +108,12 @@ __device__ inline int64_t q_offset(const RowsParams& P, int kvh, int seq_rows, i
 }
 
 template <int D>
-struct RowsShared {  // merge of an item's waves
+struct RowsShared {
   static constexpr int LP = (D < 128 ? D : 128) + 4;  // padded row
-  __align__(16) float om[4][16][LP];
+  union {
+    __align__(16) unsigned char k[4][Tile<D, 32>::BYTES];  // each wave's key block
+    __align__(16) float om[4][16][LP];                      // merge of the waves
+  };
   float sm[4][64], sl[4][64];
 };
 
@@ -119,6 +124,9 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
   constexpr int E = D < 128 ? D / 16 : 8;   // dims of a lane in a group
   constexpr int W = E / 2;
   constexpr int DG = 16 * E;                // dims of a group
+  // Cache policy of the loads: an item of 64 rows may have neighbours on the
+  // same keys; the others read their keys alone, once (non-temporal).
+  constexpr int AUX = MT == 4 ? 0 : 2;
   auto& om = sh.om;
   auto& sm = sh.sm;
   auto& sl = sh.sl;
@@ -157,27 +165,24 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
       const_cast<uint16_t*>(it.k), short(0), int(uint32_t(it.n_keys - 1) * it.kss + 2 * D), 0x00020000);
   const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint16_t*>(it.v), short(0), int(uint32_t(it.n_keys - 1) * it.vss + 2 * D), 0x00020000);
-  uint32_t koff[2], voff[8];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) koff[u] = uint32_t(16 * u + lc) * it.kss + 16u * lr;
+  using KTile = Tile<D, 32>;
+  const KTile ktile(lane, it.kss);
+  unsigned char* kl = sh.k[w];
+  uint32_t voff[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     voff[j] = uint32_t(16 * (j >> 2) + 4 * lr + (j & 3)) * it.vss + 2u * E * lc;
 
   // The scalar offset names the block's first key, which is visible: the
   // range check compares the lane offset with the records left behind it.
-  auto load_block = [&](int j0, u32x4 (&kr)[2][NKS], uint32_t (&vr)[8][VG][W]) INLINE {
-    const uint32_t ks0 = uint32_t(j0) * it.kss, vs0 = uint32_t(j0) * it.vss;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-        kr[u][ks] = __builtin_bit_cast(
-            u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, koff[u] + 64 * ks, ks0, 2));
+  u32x4 kr[KTile::NL];  // the next key block on its way to LDS
+  auto load_k = [&](int j0) INLINE { ktile.template load<AUX>(krs, uint32_t(j0) * it.kss, kr); };
+  auto load_v = [&](int j0, uint32_t (&vr)[8][VG][W]) INLINE {
+    const uint32_t vs0 = uint32_t(j0) * it.vss;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int g = 0; g < VG; ++g) load_words<W>(vrs, voff[j] + 256 * g, vs0, vr[j][g]);
+      for (int g = 0; g < VG; ++g) load_words<W, AUX>(vrs, voff[j] + 256 * g, vs0, vr[j][g]);
   };
 
   // o[mt][g][e]: lane (lc, lr) holds row lc, dims 128 g + E (4 lr + j) + e
@@ -195,18 +200,28 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
   }
   const float c = P.scale_log2;
 
-  auto block = [&](int j0, const u32x4 (&kr)[2][NKS], uint32_t (&vr)[8][VG][W]) INLINE {
+  auto block = [&](int j0, int next, uint32_t (&vr)[8][VG][W]) INLINE {
+    ktile.store(kl, kr);
+    wave_lds_fence();
+    load_k(next);
+    f32x4 st[MT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) st[mt][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4 a = KTile::operand(kl, u, lc, lr, ks);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) st[mt][u] = mfma_qk<T>(a, qb[mt][ks], st[mt][u]);
+      }
+    }
+    wave_lds_fence();
     const bool edge = CAUSAL ? j0 + 31 > it.limit : j0 + 32 > it.n_keys;
     u32x4 ph[MT], pl[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      f32x4 s[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) s[u] = mfma_qk<T>(kr[u][ks], qb[mt][ks], s[u]);
-      }
+      f32x4(&s)[2] = st[mt];
       if (SCORES && lc < it.n_rows) {  // MT == 1
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -225,8 +240,7 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
             if (CAUSAL ? j > lim[mt] || j >= it.n_keys : j >= it.n_keys) s[u][i] = -__builtin_inff();
           }
       }
-      float bm = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                       fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+      float bm = max8(s[0], s[1]);
       bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
       bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * c;
       if (__ballot(bm > m[mt] + kSlack) != 0) {
@@ -320,32 +334,35 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
       }
   };
 
-  // Wave w takes blocks first + 128 i, i < nblk, in two register sets; loads
-  // past the wave's last block repeat it, so every load is unconditional.
+  // Wave w takes blocks first + 128 i, i < nblk; a block's loads are in flight
+  // under the block before.  Loads past the wave's last block repeat it, so
+  // every load is unconditional.
   const int first = 32 * w;
   const int nblk = it.n_keys > first ? (it.n_keys - first + 127) / 128 : 0;
   auto jb = [&](int i) { return first + 128 * min(i, nblk - 1); };
-  if constexpr (D > 256) {  // one register set: q, O, K and V of a block fill the file
-    for (int i = 0; i < nblk; ++i) {
-      u32x4 ka[2][NKS];
-      uint32_t va[8][VG][W];
-      load_block(jb(i), ka, va);
-      block(jb(i), ka, va);
-    }
-  } else if (nblk > 0) {
-    u32x4 ka[2][NKS], kb[2][NKS];
-    uint32_t va[8][VG][W], vb[8][VG][W];
-    load_block(jb(0), ka, va);
-    for (int i = 0; i < nblk; i += 2) {
-      load_block(jb(i + 1), kb, vb);
-      block(jb(i), ka, va);
-      if (i + 1 >= nblk) break;
-      load_block(jb(i + 2), ka, va);
-      block(jb(i + 1), kb, vb);
+  if (nblk > 0) {
+    load_k(jb(0));
+    if constexpr (D > 256) {  // one V set: q, O, K and V of a block fill the registers
+      for (int i = 0; i < nblk; ++i) {
+        uint32_t va[8][VG][W];
+        load_v(jb(i), va);
+        block(jb(i), jb(i + 1), va);
+      }
+    } else {
+      uint32_t va[8][VG][W], vb[8][VG][W];
+      load_v(jb(0), va);
+      for (int i = 0; i < nblk; i += 2) {
+        load_v(jb(i + 1), vb);
+        block(jb(i), jb(i + 1), va);
+        if (i + 1 >= nblk) break;
+        load_v(jb(i + 2), va);
+        block(jb(i + 1), jb(i + 2), vb);
+      }
     }
   }
 
   // ---- merge the 4 waves, 16 rows and a group of dims at a time
+  __syncthreads();  // om lies where the key blocks were
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     l[mt] += __shfl_xor(l[mt], 16, 64);
@@ -405,7 +422,9 @@ __device__ inline int clamped_len(const RowsParams& P, int b) {
 // Item blockIdx.x: the prefix items first ((kv head, key range), row tile),
 // then the own-cache items ((sequence, kv head), key range, row tile).
 template <typename T, int D, int MTP, int MTO, bool CAUSAL, bool SCORES>
-__global__ __launch_bounds__(256) void rows_kernel(const RowsParams P) {
+__global__ __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(D > 128 || MTP == 4 ? 1 : 2)))
+void rows_kernel(const RowsParams P) {
   __shared__ RowsShared<D> sh;
   Item it;
   it.seq_rows = P.group * P.s_q;
@@ -413,10 +432,13 @@ __global__ __launch_bounds__(256) void rows_kernel(const RowsParams P) {
   it.raw_row = 0;
   int x = blockIdx.x;
   if (MTP > 0 && x < P.n_prefix_items) {
-    const int rt = x % P.n_rt;
-    x /= P.n_rt;
-    const int split = x % P.n_sp;
-    it.kvh = x / P.n_sp;
+    // The row tiles of one (kv head, key range) follow each other on one XCD
+    // (workgroup i runs on XCD i % 8), so its L2 serves all but the first.
+    const int y = x >> 3, rt = y % P.n_rt;
+    const int unit = (y / P.n_rt) * 8 + (x & 7);
+    if (unit >= P.kv_heads * P.n_sp) return;
+    const int split = unit % P.n_sp;
+    it.kvh = unit / P.n_sp;
     const int R = P.batch * it.seq_rows;
     const int j0 = split * P.chunk_p;
     it.k = reinterpret_cast<const uint16_t*>(P.kp) + it.kvh * P.kp_sh + int64_t(j0) * P.kp_ss;

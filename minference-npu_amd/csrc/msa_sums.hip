@@ -45,7 +45,8 @@ __device__ inline __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, int left, 
 }
 
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(256) void sums_stats_kernel(const SumsParams P) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
+void sums_stats_kernel(const SumsParams P) {
   constexpr int NKS = SumsShape<D>::NKS;
   constexpr int KB = 32;  // keys of a block
   __shared__ float sm[4][16 * MT], sl[4][16 * MT];
@@ -116,8 +117,7 @@ __global__ __launch_bounds__(256) void sums_stats_kernel(const SumsParams P) {
           for (int i = 0; i < 4; ++i)
             if (j0 + 16 * u + 4 * lr + i > last) s[u][i] = -__builtin_inff();
       }
-      const float bm = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                             fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))) * c;
+      const float bm = max8(s[0], s[1]) * c;
       if (__ballot(bm > m[mt] + 16.0f) != 0) {
         const float mn = fmaxf(m[mt], bm);
         mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
@@ -195,16 +195,29 @@ __global__ __launch_bounds__(256) void sums_stats_kernel(const SumsParams P) {
   }
 }
 
-// (m, 1 / l) of every row from its key splits.
+// (m, 1 / l) of every row from its key splits: 16 rows a workgroup, 16 threads
+// a row.
 __global__ __launch_bounds__(256) void sums_merge_kernel(const SumsParams P) {
   const int64_t n = int64_t(P.batch) * P.heads * P.s_q_pad;
-  const int64_t row = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (row >= n) return;
+  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x & 15);
+  const int g = threadIdx.x >> 4;
+  __shared__ float2 red[16][16];
   const float2* part = reinterpret_cast<const float2*>(P.part);
   float M = -__builtin_inff(), L = 0.0f;
-  for (int s = 0; s < P.n_split; ++s) M = fmaxf(M, part[s * n + row].x);
-  for (int s = 0; s < P.n_split; ++s) {
+  for (int s = g; s < P.n_split; s += 16) {
     const float2 y = part[s * n + row];
+    if (y.x == -__builtin_inff()) continue;
+    const float mn = fmaxf(M, y.x);
+    L = L * __builtin_amdgcn_exp2f(M - mn) + y.y * __builtin_amdgcn_exp2f(y.x - mn);
+    M = mn;
+  }
+  red[g][threadIdx.x & 15] = make_float2(M, L);
+  __syncthreads();
+  if (g != 0) return;
+  for (int v = 0; v < 16; ++v) M = fmaxf(M, red[v][threadIdx.x].x);
+  L = 0.0f;
+  for (int v = 0; v < 16; ++v) {
+    const float2 y = red[v][threadIdx.x];
     if (y.x != -__builtin_inff()) L += __builtin_amdgcn_exp2f(y.x - M) * y.y;
   }
   P.stat_m[row] = M == -__builtin_inff() ? 0.0f : M;
@@ -212,7 +225,8 @@ __global__ __launch_bounds__(256) void sums_merge_kernel(const SumsParams P) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void sums_cols_kernel(const SumsParams P) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
+void sums_cols_kernel(const SumsParams P) {
   constexpr int NKS = SumsShape<D>::NKS, NT = SumsShape<D>::TILES;
   constexpr int TK = 16 * NT;  // keys of a wave
   __shared__ float red[4][TK];
@@ -354,8 +368,7 @@ hipError_t launch_sums_d(const SumsParams& p, hipStream_t st) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (p.n_split > 1) {
-    hipLaunchKernelGGL(sums_merge_kernel, dim3(uint32_t((bh * p.s_q_pad + 255) / 256)), dim3(256), 0,
-                       st, p);
+    hipLaunchKernelGGL(sums_merge_kernel, dim3(uint32_t(bh * p.s_q_pad / 16)), dim3(256), 0, st, p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
