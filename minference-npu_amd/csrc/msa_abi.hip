@@ -1314,9 +1314,9 @@ int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const
   rp.s_q = int(Sq);
   rp.s_p = int(Sp);
   rp.s_c = int(Sc);
-  rp.mt = D > 128 || R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  rp.n_rt = int(cdiv(R, 16 * rp.mt));
-  rp.n_rto = int(cdiv(rows, 16));
+  rows_forms(rp, R, rows, int(D));
+  rp.n_rt = int(cdiv(R, rp.prefix_rows));
+  rp.n_rto = int(cdiv(rows, rp.own_rows));
   rows_split(Sp, std::min<int64_t>(cdiv(Sp, 256), cdiv(512, rp.n_rt * Hkv)),
              kp ? rows_max_chunk(kp, vp) : 128, rp.n_sp, rp.chunk_p);
   rows_split(Sc, std::min<int64_t>(cdiv(Sc, 256), cdiv(2048, rp.n_rto * B * Hkv)),

@@ -237,7 +237,8 @@ struct RowsParams {
   int64_t o_sb, o_sh, o_ss;
   const int32_t* lens;  // [batch] keys of each own cache, or nullptr: s_c
   int batch, heads, kv_heads, group, s_q, s_p, s_c;
-  int mt;                    // 16-row tiles of a prefix item
+  int prefix_form, own_form;  // of the items (rows_forms), and their rows
+  int prefix_rows, own_rows;
   int n_rt, n_sp, chunk_p;   // prefix: row tiles, key splits, keys of a split
   int n_rto, n_so, chunk_o;  // own caches: the same per (sequence, kv head)
   int n_prefix_items, n_items;  // prefix: (kv head, split) pairs to a multiple of 8
@@ -356,6 +357,8 @@ hipError_t launch_attention_vs(const AttnParams& p, int dtype, int out_dtype, in
 hipError_t launch_vs_build(const VsBuildParams& p, int n_bs, hipStream_t st);
 hipError_t launch_vs_estimate(const VsEstParams& p, int dtype, int D, hipStream_t st);
 hipError_t launch_block_lists(const ListParams& p, hipStream_t st);
+// Item forms of `rows` prefix rows a kv head and `seq_rows` rows of a sequence.
+void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D);
 hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,
                        hipStream_t st);
 int sums_tiles(int D);  // 16-row (16-key) tiles of a stats (columns) item

@@ -107,26 +107,93 @@ __device__ inline int64_t q_offset(const RowsParams& P, int kvh, int seq_rows, i
   return b * P.q_sb + int64_t(kvh * P.group + g) * P.q_sh + int64_t(i) * P.q_ss;
 }
 
-template <int D>
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+// V operand of 16 dims and 32 keys from LDS: 4 keys at p, 4 keys `far` bytes on.
+__device__ inline u32x4 v_operand(const unsigned char* p, int far) {
+  const u32x2 a = __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(const_cast<unsigned char*>(p))));
+  const u32x2 b = __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(const_cast<unsigned char*>(p + far))));
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// A packed pair with its Inf and NaN as 0.
+template <typename T>
+__device__ inline uint32_t finite_only(uint32_t x) {
+  constexpr uint32_t e = T::id == Bf16::id ? 0x7f80u : 0x7c00u;
+  if ((x & e) == e) x &= 0xffff0000u;
+  if ((x & (e << 16)) == (e << 16)) x &= 0xffffu;
+  return x;
+}
+
+// What the Inf and NaN values of V among the 32 keys from local key j0 add to
+// the rows that see them, one key at a time (kTile's layout of O).
+template <typename T, int MT, int ND>
+__device__ INLINE inline void add_nonfinite(const Item& it, int j0, int lane,
+                                                        const u32x4 (&ph)[MT], const u32x4 (&pl)[MT],
+                                                        const int (&lim)[MT], f32x4 (&o)[MT][ND]) {
+  const int lr = lane >> 4, lc = lane & 15;
+  for (int kk = 0; kk < 32 && j0 + kk < it.n_keys; ++kk) {
+    const uint16_t* vrow = it.v + int64_t(j0 + kk) * (it.vss / 2);
+    const int slot = 4 * (kk >> 4) + (kk & 3);  // P's place in its lane
+    const int src = lc + 16 * ((kk & 15) >> 2);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      uint32_t hw = 0, lw = 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if ((slot >> 1) == x) {
+          hw = ph[mt][x];
+          lw = pl[mt][x];
+        }
+      const float pv = (slot & 1) ? hi_of<T>(hw) + hi_of<T>(lw) : lo_of<T>(hw) + lo_of<T>(lw);
+      const float pk = __shfl(pv, src, 64);
+      const bool sees = j0 + kk <= lim[mt];
+#pragma unroll
+      for (int n = 0; n < ND; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = T::to_float(vrow[16 * n + 4 * lr + i]);
+          if (sees && !__builtin_isfinite(x)) o[mt][n][i] += pk * x;
+        }
+    }
+  }
+}
+
+// Forms of an item: kOwn + MT: up to 16 MT rows, the four waves take different
+// keys; kTile + MT: up to 64 MT rows, 16 MT a wave, the waves share the keys.
+constexpr int kOwn = 0, kTile = 8;
+constexpr int form_rows(int form) {
+  return form >= kTile ? 64 * (form - kTile) : 16 * form;
+}
+constexpr int kTileKeys = 64;
+
+// Bytes between V rows of a tile in LDS: 8 rows that a half wave reads 32 bytes
+// of each lie in 8 different groups of 8 banks.
+constexpr int v_row_bytes(int D) { return 2 * D + 32; }
+
+template <int D, int FORMS>  // FORMS: 1 when a tile form is among them
 struct RowsShared {
   static constexpr int LP = (D < 128 ? D : 128) + 4;  // padded row
+  static constexpr int STAGE = FORMS ? kTileKeys * (2 * D + v_row_bytes(D)) : 16;
   union {
-    __align__(16) unsigned char k[4][Tile<D, 32>::BYTES];  // each wave's key block
-    __align__(16) float om[4][16][LP];                      // merge of the waves
+    __align__(16) unsigned char k[4][Tile<D, 32>::BYTES];  // kOwn: each wave's key block
+    __align__(16) float om[4][16][LP];                      // kOwn: merge of the waves
+    __align__(16) unsigned char kv[2][STAGE];               // kTile: K and V of two tiles
   };
-  float sm[4][64], sl[4][64];
+  float sm[4][32], sl[4][32];
 };
 
-template <typename T, int D, int MT, bool CAUSAL, bool SCORES>
-__device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh) {
+template <typename T, int D, int MT, bool CAUSAL, bool SCORES, typename Shared>
+__device__ void rows_item(const RowsParams& P, const Item& it, Shared& sh) {
   constexpr int NKS = D / 32;
   constexpr int VG = (D + 127) / 128;       // groups of 128 dims of V
   constexpr int E = D < 128 ? D / 16 : 8;   // dims of a lane in a group
   constexpr int W = E / 2;
   constexpr int DG = 16 * E;                // dims of a group
-  // Cache policy of the loads: an item of 64 rows may have neighbours on the
-  // same keys; the others read their keys alone, once (non-temporal).
-  constexpr int AUX = MT == 4 ? 0 : 2;
+  constexpr int AUX = 2;  // the item reads its keys alone, once: non-temporal loads
   auto& om = sh.om;
   auto& sm = sh.sm;
   auto& sl = sh.sl;
@@ -278,15 +345,13 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
 #pragma unroll
           for (int x = 0; x < W; ++x) bad |= any_nonfinite<T>(vr[j][g][x]);
       if (__ballot(bad) != 0) {
-        constexpr uint32_t ex = T::id == Bf16::id ? 0x7f80u : 0x7c00u;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
           for (int g = 0; g < VG; ++g)
 #pragma unroll
             for (int x = 0; x < W; ++x) {
-              if ((vr[j][g][x] & ex) == ex) vr[j][g][x] &= 0xffff0000u;
-              if ((vr[j][g][x] & (ex << 16)) == (ex << 16)) vr[j][g][x] &= 0xffffu;
+              vr[j][g][x] = finite_only<T>(vr[j][g][x]);
             }
         for (int kk = 0; kk < 32 && j0 + kk < it.n_keys; ++kk) {
           const uint16_t* vrow = it.v + int64_t(j0 + kk) * (it.vss / 2);
@@ -415,23 +480,211 @@ __device__ void rows_item(const RowsParams& P, const Item& it, RowsShared<D>& sh
   }
 }
 
+// kTile: 64 keys of K and V at a time in LDS for the four waves, the next tile
+// on its way through registers.  V operands are transposing LDS reads: a group of
+// 16 lanes takes 4 keys of 16 dims, which is the key order of P.
+template <typename T, int D, int MT, bool CAUSAL, typename Shared>
+__device__ void rows_tile_item(const RowsParams& P, const Item& it, Shared& sh) {
+  constexpr int NKS = D / 32, ND = D / 16;
+  constexpr int VS = v_row_bytes(D);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int lr = lane >> 4;
+  const int lc = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  if (it.n_keys <= 0) {
+    for (int r = tid; r < it.n_rows; r += 256) {
+      P.ml[2 * (it.part_row + r)] = -__builtin_inff();
+      P.ml[2 * (it.part_row + r) + 1] = 0.0f;
+    }
+    return;
+  }
+  const int wr0 = 16 * MT * w;  // first row of this wave in the item
+  const bool active = wr0 < it.n_rows;
+
+  u32x4 qb[MT][NKS];
+  int lim[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = it.row0 + min(wr0 + 16 * mt + lc, it.n_rows - 1);
+    const uint16_t* qrow =
+        reinterpret_cast<const uint16_t*>(P.q) + q_offset(P, it.kvh, it.seq_rows, r);
+#pragma unroll
+    for (int ks = 0; ks < NKS; ++ks) qb[mt][ks] = load16(qrow + 32 * ks + 8 * lr);
+    lim[mt] = CAUSAL ? it.limit + r % P.s_q : 0;
+  }
+
+  const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(it.k), short(0), int(uint32_t(it.n_keys - 1) * it.kss + 2 * D), 0x00020000);
+  const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<uint16_t*>(it.v), short(0), int(uint32_t(it.n_keys - 1) * it.vss + 2 * D), 0x00020000);
+  // this wave stages 16 of the tile's 64 rows
+  using Part = Tile<D, 16>;
+  const Part kpart(lane, it.kss), vpart(lane, it.vss);
+  u32x4 kr[Part::NL], vr[Part::NL];
+  auto load_tile = [&](int j0) INLINE {
+    kpart.load_at(krs, uint32_t(j0 + 16 * w) * it.kss, kr);
+    vpart.load_at(vrs, uint32_t(j0 + 16 * w) * it.vss, vr);
+  };
+  auto store_tile = [&](unsigned char* stage) INLINE {
+    kpart.store(stage + w * Part::BYTES, kr);
+    unsigned char* vl = stage + 4 * Part::BYTES + 16 * w * VS;
+#pragma unroll
+    for (int i = 0; i < Part::NL; ++i) {
+      const int f = 64 * i + lane, r = f / Part::NCH, c = f - r * Part::NCH;
+      *reinterpret_cast<u32x4*>(vl + r * VS + 16 * c) = vr[i];
+    }
+  };
+
+  // o[mt][n]: lane (lc, lr) holds row lc, dims 16 n + 4 lr + i
+  f32x4 o[MT][ND];
+  float m[MT], mp[MT], l[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = -__builtin_inff();
+    mp[mt] = 0.0f;
+    l[mt] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < ND; ++n) o[mt][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const float c = P.scale_log2;
+
+  // 32 keys of a tile: from local key j0, rows 32 h .. of the stage
+  auto block = [&](int j0, const unsigned char* stage, int h) INLINE {
+    const bool edge = CAUSAL ? j0 + 31 > it.limit : j0 + 32 > it.n_keys;
+    f32x4 st[MT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) st[mt][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4 a = Part::operand(stage + (2 * h + u) * Part::BYTES, 0, lc, lr, ks);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) st[mt][u] = mfma_qk<T>(a, qb[mt][ks], st[mt][u]);
+      }
+    }
+    u32x4 ph[MT], pl[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      f32x4(&s)[2] = st[mt];
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = j0 + 16 * u + 4 * lr + i;
+            if ((CAUSAL && j > lim[mt]) || j >= it.n_keys) s[u][i] = -__builtin_inff();
+          }
+      }
+      float bm = max8(s[0], s[1]);
+      bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+      bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * c;
+      if (__ballot(bm > m[mt] + kSlack) != 0) {
+        const float mn = fmaxf(m[mt], bm);
+        mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
+        const float al = __builtin_amdgcn_exp2f(m[mt] - mp[mt]);
+        m[mt] = mn;
+        l[mt] *= al;
+#pragma unroll
+        for (int n = 0; n < ND; ++n) o[mt][n] *= al;
+      }
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], c, -mp[mt]));
+      l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ph[mt][j] = pack2<T>(p[2 * j], p[2 * j + 1]);
+        pl[mt][j] = pack2<T>(p[2 * j] - lo_of<T>(ph[mt][j]), p[2 * j + 1] - hi_of<T>(ph[mt][j]));
+      }
+    }
+    const unsigned char* vl = stage + 4 * Part::BYTES + (32 * h + 4 * lr + (lc >> 2)) * VS + 8 * (lc & 3);
+    bool bad = false;
+    if (CAUSAL && edge) {  // as in rows_item
+#pragma unroll
+      for (int n = 0; n < ND; ++n) {
+        const u32x4 a = v_operand(vl + 32 * n, 16 * VS);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) bad |= any_nonfinite<T>(a[x]);
+      }
+      bad = __ballot(bad) != 0;
+      if (bad) add_nonfinite<T, MT, ND>(it, j0, lane, ph, pl, lim, o);
+    }
+#pragma unroll
+    for (int n = 0; n < ND; ++n) {
+      u32x4 a = v_operand(vl + 32 * n, 16 * VS);
+      if (CAUSAL && bad) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) a[x] = finite_only<T>(a[x]);
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        o[mt][n] = mfma_qk<T>(a, ph[mt], o[mt][n]);
+        o[mt][n] = mfma_qk<T>(a, pl[mt], o[mt][n]);
+      }
+    }
+  };
+
+  const int nt = (it.n_keys + kTileKeys - 1) / kTileKeys;
+  load_tile(0);
+  store_tile(sh.kv[0]);
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    // rows behind the last tile read 0 and are not used
+    load_tile(kTileKeys * (t + 1));
+    if (active) {
+      block(kTileKeys * t, sh.kv[t & 1], 0);
+      if (kTileKeys * t + 32 < it.n_keys) block(kTileKeys * t + 32, sh.kv[t & 1], 1);
+    }
+    store_tile(sh.kv[(t + 1) & 1]);
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    l[mt] += __shfl_xor(l[mt], 16, 64);
+    l[mt] += __shfl_xor(l[mt], 32, 64);
+    const int row = wr0 + 16 * mt + lc;
+    if (row >= it.n_rows) continue;
+    const int64_t pr = it.part_row + row;
+#pragma unroll
+    for (int n = 0; n < ND; ++n)
+      *reinterpret_cast<f32x4*>(P.part + pr * D + 16 * n + 4 * lr) = o[mt][n];
+    if (lr == 0) {
+      P.ml[2 * pr] = m[mt];
+      P.ml[2 * pr + 1] = l[mt];
+    }
+  }
+}
+
 __device__ inline int clamped_len(const RowsParams& P, int b) {
   return P.lens ? max(0, min(P.lens[b], P.s_c)) : P.s_c;
 }
 
-// Item blockIdx.x: the prefix items first ((kv head, key range), row tile),
-// then the own-cache items ((sequence, kv head), key range, row tile).
-template <typename T, int D, int MTP, int MTO, bool CAUSAL, bool SCORES>
-__global__ __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(D > 128 || MTP == 4 ? 1 : 2)))
+template <typename T, int D, int FORM, bool CAUSAL, bool SCORES, typename Shared>
+__device__ inline void run_item(const RowsParams& P, const Item& it, Shared& sh) {
+  if constexpr (FORM >= kTile)
+    rows_tile_item<T, D, FORM - kTile, CAUSAL>(P, it, sh);
+  else
+    rows_item<T, D, FORM, CAUSAL, SCORES>(P, it, sh);
+}
+
+// Item blockIdx.x: the prefix items first ((kv head, key range), row tile) in
+// form PF (0: none), then the own-cache items ((sequence, kv head), key range,
+// row tile) in form OF.
+template <typename T, int D, int PF, int OF, bool CAUSAL, bool SCORES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2)))
 void rows_kernel(const RowsParams P) {
-  __shared__ RowsShared<D> sh;
+  __shared__ RowsShared<D, (PF >= kTile || OF >= kTile)> sh;
   Item it;
   it.seq_rows = P.group * P.s_q;
   it.raw = nullptr;
   it.raw_row = 0;
   int x = blockIdx.x;
-  if (MTP > 0 && x < P.n_prefix_items) {
+  if (PF > 0 && x < P.n_prefix_items) {
     // The row tiles of one (kv head, key range) follow each other on one XCD
     // (workgroup i runs on XCD i % 8), so its L2 serves all but the first.
     const int y = x >> 3, rt = y % P.n_rt;
@@ -447,10 +700,10 @@ void rows_kernel(const RowsParams P) {
     it.vss = uint32_t(P.vp_ss) * 2u;
     it.n_keys = min(P.chunk_p, P.s_p - j0);
     it.limit = 0;
-    it.row0 = rt * 16 * MTP;
-    it.n_rows = min(16 * MTP, R - it.row0);
+    it.row0 = rt * form_rows(PF);
+    it.n_rows = min(form_rows(PF), R - it.row0);
     it.part_row = (int64_t(it.kvh) * P.n_sp + split) * R + it.row0;
-    if constexpr (MTP > 0) rows_item<T, D, MTP, false, false>(P, it, sh);
+    if constexpr (PF > 0) run_item<T, D, PF, false, false>(P, it, sh);
     return;
   }
   x -= P.n_prefix_items;
@@ -468,15 +721,15 @@ void rows_kernel(const RowsParams P) {
   it.vss = uint32_t(P.v_ss) * 2u;
   it.n_keys = min(P.chunk_o, len - j0);
   it.limit = len - P.s_q - j0;
-  const int r0 = rt * 16 * MTO;
+  const int r0 = rt * form_rows(OF);
   it.row0 = b * it.seq_rows + r0;
-  it.n_rows = min(16 * MTO, it.seq_rows - r0);
+  it.n_rows = min(form_rows(OF), it.seq_rows - r0);
   it.part_row = P.own_row0 + (int64_t(b * P.kv_heads + it.kvh) * P.n_so + split) * it.seq_rows + r0;
   if constexpr (SCORES) {  // s_q == 1: rows are the heads of the group
     it.raw_row = P.s_c;
     it.raw = P.raw + (int64_t(b) * P.heads + it.kvh * P.group + r0) * P.s_c + j0;
   }
-  rows_item<T, D, MTO, CAUSAL, SCORES>(P, it, sh);
+  run_item<T, D, OF, CAUSAL, SCORES>(P, it, sh);
 }
 
 template <typename T, bool OUT_F32>
@@ -619,11 +872,28 @@ __global__ __launch_bounds__(256) void rows_weights_kernel(const RowsParams P, i
   }
 }
 
-template <typename T, bool OUT_F32, int D, int MTP, int MTO, bool CAUSAL>
-hipError_t launch_prefix_k(const RowsParams& p, hipStream_t st) {
+template <typename T, int D, int PF, int OF, bool CAUSAL>
+void launch_prefix_k(const RowsParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((rows_kernel<T, D, PF, OF, CAUSAL, false>), dim3(p.n_items), dim3(256), 0, st, p);
+}
+
+template <typename T, int D, bool CAUSAL>
+void launch_prefix_f(const RowsParams& p, hipStream_t st) {
+  if constexpr (D <= 128) {
+    if constexpr (CAUSAL)
+      if (p.own_form == kTile + 2) return launch_prefix_k<T, D, kTile + 2, kTile + 2, true>(p, st);
+    if (p.prefix_form == kTile + 2) return launch_prefix_k<T, D, kTile + 2, kOwn + 1, CAUSAL>(p, st);
+    if (p.prefix_form == kTile + 1) return launch_prefix_k<T, D, kTile + 1, kOwn + 1, CAUSAL>(p, st);
+    if (p.prefix_form == kOwn + 2) return launch_prefix_k<T, D, kOwn + 2, kOwn + 1, CAUSAL>(p, st);
+  }
+  launch_prefix_k<T, D, kOwn + 1, kOwn + 1, CAUSAL>(p, st);
+}
+
+template <typename T, bool OUT_F32, int D>
+hipError_t launch_prefix_d(const RowsParams& p, hipStream_t st) {
   if (p.n_items > 0) {
-    hipLaunchKernelGGL((rows_kernel<T, D, MTP, MTO, CAUSAL, false>), dim3(p.n_items), dim3(256), 0,
-                       st, p);
+    if (p.s_q == 1) launch_prefix_f<T, D, false>(p, st);
+    else launch_prefix_f<T, D, true>(p, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -633,25 +903,9 @@ hipError_t launch_prefix_k(const RowsParams& p, hipStream_t st) {
 }
 
 template <typename T, bool OUT_F32, int D>
-hipError_t launch_prefix_d(const RowsParams& p, hipStream_t st) {
-  if constexpr (D <= 128) {
-    if (p.s_q == 1)
-      return p.mt == 4   ? launch_prefix_k<T, OUT_F32, D, 4, 1, false>(p, st)
-             : p.mt == 2 ? launch_prefix_k<T, OUT_F32, D, 2, 1, false>(p, st)
-                         : launch_prefix_k<T, OUT_F32, D, 1, 1, false>(p, st);
-    return p.mt == 4   ? launch_prefix_k<T, OUT_F32, D, 4, 1, true>(p, st)
-           : p.mt == 2 ? launch_prefix_k<T, OUT_F32, D, 2, 1, true>(p, st)
-                       : launch_prefix_k<T, OUT_F32, D, 1, 1, true>(p, st);
-  } else {
-    return p.s_q == 1 ? launch_prefix_k<T, OUT_F32, D, 1, 1, false>(p, st)
-                      : launch_prefix_k<T, OUT_F32, D, 1, 1, true>(p, st);
-  }
-}
-
-template <typename T, bool OUT_F32, int D>
 hipError_t launch_accumulate_d(const RowsParams& p, hipStream_t st) {
   if (p.n_items > 0) {
-    hipLaunchKernelGGL((rows_kernel<T, D, 0, 1, false, true>), dim3(p.n_items), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((rows_kernel<T, D, 0, kOwn + 1, false, true>), dim3(p.n_items), dim3(256), 0, st, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -677,6 +931,18 @@ hipError_t launch_rows_t(const RowsParams& p, bool accumulate, int D, hipStream_
 }
 
 }  // namespace
+
+void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D) {
+  const bool tiles = D <= 128;
+  p.own_form = tiles && p.s_q > 1 && seq_rows > 32 ? kTile + 2 : kOwn + 1;
+  p.prefix_form = !tiles || rows <= 16       ? kOwn + 1
+                  : p.own_form > kTile       ? kTile + 2
+                  : rows <= 32               ? kOwn + 2
+                  : rows <= 64               ? kTile + 1
+                                             : kTile + 2;
+  p.prefix_rows = form_rows(p.prefix_form);
+  p.own_rows = form_rows(p.own_form);
+}
 
 hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,
                        hipStream_t st) {

@@ -54,6 +54,13 @@ struct Tile {
       x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off[i], soff, AUX));
   }
 
+  // The same without a scalar offset: base may lie behind the descriptor's end.
+  __device__ void load_at(__amdgpu_buffer_rsrc_t rs, uint32_t base, u32x4 (&x)[NL]) const {
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, base + off[i], 0, 0));
+  }
+
   __device__ void store(unsigned char* lds, const u32x4 (&x)[NL]) const {
 #pragma unroll
     for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4*>(lds + put[i]) = x[i];

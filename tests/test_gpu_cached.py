@@ -61,6 +61,9 @@ PREFIX = [
     (2, 4, 2, 96, 0, 40, 1, BF16, [40, 0]),             # no prefix, an empty sequence
     (2, 4, 2, 96, 50, 0, 1, BF16, None),                # no own cache
     (2, 4, 2, 64, 0, 30, 4, FP16, [30, 2]),             # rows that see nothing
+    (3, 16, 1, 64, 700, 33, 1, BF16, [33, 32, 1]),      # 48 rows
+    (7, 16, 1, 128, 300, 100, 1, FP16, None),           # 112 rows
+    (2, 8, 1, 96, 65, 130, 20, FP16, [130, 97]),        # 160 rows of a sequence
     (1, 8, 8, 96, 20000, 600, 1, BF16, None),
     (2, 2, 2, 128, 9000, 300, 40, BF16, [300, 150]),
 ]
@@ -113,16 +116,17 @@ def test_shared_prefix_strided_views(gpu_device):
 
 
 @pytest.mark.parametrize("dt", [BF16, FP16])
-def test_shared_prefix_nonfinite_values(gpu_device, dt):
+@pytest.mark.parametrize("Sq", [6, 40])
+def test_shared_prefix_nonfinite_values(gpu_device, dt, Sq):
     """An Inf or NaN in V reaches the rows that see its key and no others;
     +-Inf and NaN keys behave as in softmax."""
     from minference import shared_prefix_attention
 
-    B, H, Hkv, D, Sp, Sc, Sq = 2, 4, 2, 96, 40, 50, 6
+    B, H, Hkv, D, Sp, Sc = 2, 4, 2, 96, 40, 50
     q, kp, vp = rand(1, B, H, Sq, D, dtype=dt), rand(2, 1, Hkv, Sp, D, dtype=dt), rand(3, 1, Hkv, Sp, D, dtype=dt)
     k, v = rand(4, B, Hkv, Sc, D, dtype=dt), rand(5, B, Hkv, Sc, D, dtype=dt)
     lens = [50, 33]
-    v[0, 0, 47, 5] = float("inf")   # rows 0..2 of sequence 0 do not see it
+    v[0, 0, 47, 5] = float("inf")   # the first rows of sequence 0 do not see it
     v[0, 0, 49, 17] = float("nan")  # only the last row sees it
     v[1, 1, 30, 3] = float("-inf")
     ref = O.shared_prefix(q, kp, vp, k, v, lens, D ** -0.5)
