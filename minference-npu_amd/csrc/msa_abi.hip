@@ -1510,21 +1510,19 @@ int sums_plan(SumsParams& sp, SumsLayout& l, const msa_tensor4* q, const msa_ten
   sp.s_k = int(Sk);
   sp.s_q_pad = int(cdiv(Sq, 16) * 16);
   const int tiles = sums_tiles(int(D));
-  sp.mt = Sq <= 16 ? 1 : tiles;
-  sp.n_rt = int(cdiv(Sq, 16 * sp.mt));
-  // stats: key splits where there are few row tiles
+  sp.share = Sq > 16 * tiles;
+  sp.stat_rows = sp.share ? 64 * tiles : Sq <= 16 ? 16 : 16 * tiles;
+  sp.n_rt = int(cdiv(Sq, sp.stat_rows));
+  // stats: key splits where there are few items
   const int64_t items = BH * sp.n_rt;
   const int64_t want = std::min<int64_t>(cdiv(Sk, 512), cdiv(1024, items));
   sp.chunk = int(cdiv(cdiv(Sk, want), 128) * 128);
   sp.n_split = items >= 512 ? 1 : int(cdiv(Sk, sp.chunk));
   if (sp.n_split == 1) sp.chunk = int(cdiv(Sk, 128) * 128);
-  // columns: a key tile per wave where there are few rows for four waves; row
-  // splits where there are few key tiles
-  const int64_t blocks = sp.s_q_pad / 16 * sp.group;  // 16-row blocks of the first keys
-  sp.wave_keys = blocks < 64 && B * Hkv * cdiv(Sk, 64 * tiles) >= 512;
-  sp.n_kt = int(cdiv(Sk, 16 * tiles * (sp.wave_keys ? 4 : 1)));
-  const int64_t ci = B * Hkv * sp.n_kt;
-  sp.n_rsplit = ci >= 512 ? 1 : int(std::max<int64_t>(1, std::min(cdiv(1024, ci), blocks / 16)));
+  // columns: row splits where there are few items, of at least 8 tiles of 64 rows
+  sp.n_kt = int(cdiv(Sk, 64 * tiles));
+  const int64_t ci = B * Hkv * sp.n_kt, row_tiles = cdiv(Sq, 64) * sp.group;
+  sp.n_rsplit = int(std::max<int64_t>(1, std::min(cdiv(2048, ci), row_tiles / 8)));
   if (items * sp.n_split >= (int64_t(1) << 31) || ci * sp.n_rsplit >= (int64_t(1) << 31) ||
       B * Hkv > 65535)
     return MSA_E_HEADS;

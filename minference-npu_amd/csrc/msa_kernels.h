@@ -264,8 +264,9 @@ struct SumsParams {
   int add;        // 1: added to what is there
   int batch, heads, kv_heads, group, s_q, s_k, s_q_pad;  // s_q_pad: s_q to 16
   float scale_log2;
-  int mt, n_rt, n_split, chunk;   // stats: row tiles of an item, items, key splits
-  int n_kt, n_rsplit, wave_keys;  // columns: key tiles, row splits; 1: a key tile per wave
+  int share, stat_rows;       // stats: waves on different rows (1) or keys (0), rows of an item
+  int n_rt, n_split, chunk;   // items of a head, key splits, keys of a split
+  int n_kt, n_rsplit;         // columns: key tiles of an item's four waves, row splits
   float* part;      // n_split > 1: (m, l) [n_split][batch * heads][s_q_pad]
   float* stat_m;    // [batch * heads][s_q_pad]: max of the row's scores, log2 units
   float* stat_r;    // 1 / sum

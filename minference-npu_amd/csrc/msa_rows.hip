@@ -307,10 +307,11 @@ __device__ void rows_item(const RowsParams& P, const Item& it, Shared& sh) {
             if (CAUSAL ? j > lim[mt] || j >= it.n_keys : j >= it.n_keys) s[u][i] = -__builtin_inff();
           }
       }
-      float bm = max8(s[0], s[1]);
-      bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * c;
+      // the lanes of a row compare their own keys; they only exchange to move it
+      float bm = max8(s[0], s[1]) * c;
       if (__ballot(bm > m[mt] + kSlack) != 0) {
+        bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+        bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
         const float mn = fmaxf(m[mt], bm);
         mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
         const float al = __builtin_amdgcn_exp2f(m[mt] - mp[mt]);  // m = -inf at first: 0
@@ -323,14 +324,14 @@ __device__ void rows_item(const RowsParams& P, const Item& it, Shared& sh) {
       }
       float p[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 8; ++j)
         p[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], c, -mp[mt]));
-        l[mt] += p[j];
-      }
+      l[mt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         ph[mt][j] = pack2<T>(p[2 * j], p[2 * j + 1]);
-        pl[mt][j] = pack2<T>(p[2 * j] - lo_of<T>(ph[mt][j]), p[2 * j + 1] - hi_of<T>(ph[mt][j]));
+        pl[mt][j] = pack2<T>(__builtin_fmaf(lo_of<T>(ph[mt][j]), -1.0f, p[2 * j]),
+                             __builtin_fmaf(hi_of<T>(ph[mt][j]), -1.0f, p[2 * j + 1]));
       }
     }
     if (CAUSAL && edge) {
@@ -578,10 +579,11 @@ __device__ void rows_tile_item(const RowsParams& P, const Item& it, Shared& sh) 
             if ((CAUSAL && j > lim[mt]) || j >= it.n_keys) s[u][i] = -__builtin_inff();
           }
       }
-      float bm = max8(s[0], s[1]);
-      bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
-      bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * c;
+      // the lanes of a row compare their own keys; they only exchange to move it
+      float bm = max8(s[0], s[1]) * c;
       if (__ballot(bm > m[mt] + kSlack) != 0) {
+        bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
+        bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
         const float mn = fmaxf(m[mt], bm);
         mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
         const float al = __builtin_amdgcn_exp2f(m[mt] - mp[mt]);
@@ -598,7 +600,8 @@ __device__ void rows_tile_item(const RowsParams& P, const Item& it, Shared& sh) 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         ph[mt][j] = pack2<T>(p[2 * j], p[2 * j + 1]);
-        pl[mt][j] = pack2<T>(p[2 * j] - lo_of<T>(ph[mt][j]), p[2 * j + 1] - hi_of<T>(ph[mt][j]));
+        pl[mt][j] = pack2<T>(__builtin_fmaf(lo_of<T>(ph[mt][j]), -1.0f, p[2 * j]),
+                             __builtin_fmaf(hi_of<T>(ph[mt][j]), -1.0f, p[2 * j + 1]));
       }
     }
     const unsigned char* vl = stage + 4 * Part::BYTES + (32 * h + 4 * lr + (lc >> 2)) * VS + 8 * (lc & 3);

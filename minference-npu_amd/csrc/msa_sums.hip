@@ -6,22 +6,23 @@
 //
 // A weight needs its row's maximum and sum over all keys, a column sum needs
 // the weights of all rows, so q.k is taken twice:
-//   stats: an item holds up to 64 rows of a head as the B operand and walks the
+//   stats: a wave holds up to 64 rows of a head as the B operand and walks the
 //     keys: S^T = K . Q^T, lane (lc, lr) gets row lc, keys 4 lr + i.  Each lane
 //     keeps a running (m, l) of the keys it sees: no exchange until the end.
-//   columns: an item holds 64 keys of a kv head as the B operand and walks the
+//   columns: a wave holds 64 keys of a kv head as the B operand and walks the
 //     rows of all its heads: S = Q . K^T, lane (lc, lr) gets key lc, rows 4 lr +
-//     i, whose (m, 1 / l) are one 32-byte read.  Each lane sums its keys' weights
-//     in registers.
-// No LDS in the loops.  Bound by the exponentials, two for each visible pair (a
-// quarter-rate instruction), with the products beside them: q.k costs a 16x16
-// tile D / 32 MFMAs, its 256 weights a fused multiply-add, an exponential and
-// an add a lane four times.
-// Sums are fp32 in two levels (16 blocks of 16 rows, then those), in a fixed
-// order.
+//     i.  Each lane sums its keys' weights in registers.
+// The walked rows go through LDS, 64 a tile, for the four waves of a workgroup
+// (256 rows or keys); with at most 64 rows in all the waves of a stats item
+// take different keys instead.  The scores of the next 32 rows are multiplied
+// while the exponentials of the last 32 are taken.
+// Bound by the exponentials, two for each visible pair (a quarter-rate
+// instruction), with a fused multiply-add and an add beside each.
+// Sums are fp32 in two levels, in a fixed order.
 
 #include "msa_common.h"
 #include "msa_kernels.h"
+#include "msa_tile.h"
 
 namespace msa {
 
@@ -29,26 +30,55 @@ namespace msa {
 
 namespace {
 
+constexpr int kTileRows = 64;  // walked rows (keys) of a tile in LDS
+
 template <int D>
 struct SumsShape {
   static constexpr int NKS = D / 32;
-  static constexpr int TILES = D <= 128 ? 4 : D == 256 ? 2 : 1;  // 16-row tiles held by an item
+  static constexpr int TILES = D <= 128 ? 4 : D == 256 ? 2 : 1;  // 16-row tiles a wave holds
+  using Part = Tile<D, 16>;                                      // a wave's share of a tile
+  static constexpr int STAGE = 4 * Part::BYTES;
 };
 
-// Descriptor of up to `rows` rows from `p` on, `left` of which exist (at least
-// one): loads of the others return 0.
+// Descriptor of up to `rows` rows from `p` on, `left` of which exist: loads of
+// the others return 0.
 __device__ inline __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, int left, int rows,
                                                    uint32_t stride, int D) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), short(0),
-                                           int(uint32_t(min(left, rows) - 1) * stride + 2 * D),
-                                           0x00020000);
+  const uint32_t n = left > 0 ? uint32_t(min(left, rows) - 1) * stride + 2 * D : 0u;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), short(0), int(n), 0x00020000);
 }
 
-template <typename T, int D, int MT>
+// Operands of the 16 MT rows from `p` on (`left` exist, the others are 0),
+// through this wave's 16 rows of LDS.
+template <int D, int MT>
+__device__ inline void hold_rows(const uint16_t* p, int left, int64_t stride, int lane,
+                                 unsigned char* lds, u32x4 (&x)[MT][D / 32]) {
+  using Part = Tile<D, 16>;
+  const Part part(lane, uint32_t(stride) * 2u);
+  u32x4 r[MT][Part::NL];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+    part.load_at(rows_rsrc(p + 16 * mt * stride, left - 16 * mt, 16, uint32_t(stride) * 2u, D), 0, r[mt]);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    part.store(lds, r[mt]);
+    wave_lds_fence();
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks)
+      x[mt][ks] = Part::operand(lds, 0, lane & 15, lane >> 4, ks);
+    wave_lds_fence();
+  }
+}
+
+// SHARE: four waves of 16 MT rows each against the same keys; otherwise one set
+// of rows, the waves on different keys.
+template <typename T, int D, int MT, bool SHARE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
 void sums_stats_kernel(const SumsParams P) {
-  constexpr int NKS = SumsShape<D>::NKS;
-  constexpr int KB = 32;  // keys of a block
+  using Shape = SumsShape<D>;
+  using Part = typename Shape::Part;
+  constexpr int NKS = Shape::NKS;
+  __shared__ __align__(16) unsigned char lds[2 * Shape::STAGE];
   __shared__ float sm[4][16 * MT], sl[4][16 * MT];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane >> 4, lc = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -59,107 +89,185 @@ void sums_stats_kernel(const SumsParams P) {
   const int split = x % P.n_split;
   const int rt = P.n_rt - 1 - x / P.n_split;
   const int b = bh / P.heads, h = bh - b * P.heads;
-  const int row0 = rt * 16 * MT;
-  const int n_rows = min(16 * MT, P.s_q - row0);
+  const int wg_row0 = rt * 16 * MT * (SHARE ? 4 : 1);
+  const int row0 = wg_row0 + (SHARE ? 16 * MT * w : 0);  // of this wave
+  const int wg_rows = min(16 * MT * (SHARE ? 4 : 1), P.s_q - wg_row0);
   const int shift = P.s_k - P.s_q;
   const int j_begin = split * P.chunk;
-  const int j_end = min(min(j_begin + P.chunk, P.s_k), shift + row0 + n_rows);
+  const int j_end = min(min(j_begin + P.chunk, P.s_k), shift + wg_row0 + wg_rows);
+  const int n_tiles = j_end > j_begin ? (j_end - j_begin + kTileRows - 1) / kTileRows : 0;
 
   u32x4 qb[MT][NKS];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const uint16_t* qrow = reinterpret_cast<const uint16_t*>(P.q) + b * P.q_sb + int64_t(h) * P.q_sh +
-                           int64_t(row0 + min(16 * mt + lc, n_rows - 1)) * P.q_ss;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) qb[mt][ks] = load16(qrow + 32 * ks + 8 * lr);
-  }
+  hold_rows<D, MT>(reinterpret_cast<const uint16_t*>(P.q) + b * P.q_sb + int64_t(h) * P.q_sh +
+                       int64_t(min(row0, P.s_q - 1)) * P.q_ss,
+                   P.s_q - row0, P.q_ss, lane, lds + w * Part::BYTES, qb);
+
   const uint16_t* kbase = reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb +
                           int64_t(h / P.group) * P.k_sh;
   const uint32_t kss = uint32_t(P.k_ss) * 2u;
-  const uint32_t koff = uint32_t(lc) * kss + 16u * lr;
-  auto load_block = [&](int j0, u32x4 (&kr)[2][NKS]) INLINE {
-    const __amdgpu_buffer_rsrc_t rs =
-        rows_rsrc(kbase + int64_t(j0) * P.k_ss, P.s_k - j0, KB, kss, D);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-        kr[u][ks] = __builtin_bit_cast(
-            u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, koff + 16u * u * kss + 64 * ks, 0, 0));
-  };
+  const Part part(lane, kss);
 
-  // of the keys this lane sees: running max, what the exponentials are taken
-  // against, and the sum in two levels (small terms are not lost in a long sum)
-  float m[MT], mp[MT], l[MT], part[MT];
+  // of the keys this lane sees: what the exponentials are taken against (a
+  // score of the row, at most 2^64 below the largest), and the sum in two
+  // levels (small terms are not lost in a long sum)
+  float mp[MT], l[MT], acc[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    m[mt] = -__builtin_inff();
-    mp[mt] = 0.0f;
-    l[mt] = part[mt] = 0.0f;
+    mp[mt] = -__builtin_inff();
+    l[mt] = acc[mt] = 0.0f;
   }
   const float c = P.scale_log2;
-  auto block = [&](int j0, const u32x4 (&kr)[2][NKS]) INLINE {
-    const bool edge = j0 + KB - 1 > shift + row0;  // some row does not see the whole block
+  auto scores = [&](const unsigned char* lp, f32x4 (&s)[MT][2]) INLINE {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      f32x4 s[2];
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int mt = 0; mt < MT; ++mt) s[mt][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) s[u] = mfma_qk<T>(kr[u][ks], qb[mt][ks], s[u]);
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4 a = Part::operand(lp + u * Part::BYTES, 0, lc, lr, ks);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][u] = mfma_qk<T>(a, qb[mt][ks], s[mt][u]);
       }
-      if (edge) {
+    }
+  };
+  // Hides what a row does not see, and starts the reference of a lane that has
+  // none yet.
+  auto prepare = [&](int j0, f32x4 (&s)[MT][2]) INLINE {
+    if (j0 + 31 > shift + row0 || j0 + 32 > j_end) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
         const int last = min(shift + row0 + 16 * mt + lc, j_end - 1);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (j0 + 16 * u + 4 * lr + i > last) s[u][i] = -__builtin_inff();
+            if (j0 + 16 * u + 4 * lr + i > last) s[mt][u][i] = -__builtin_inff();
       }
-      const float bm = max8(s[0], s[1]) * c;
-      if (__ballot(bm > m[mt] + 16.0f) != 0) {
-        const float mn = fmaxf(m[mt], bm);
-        mp[mt] = mn == -__builtin_inff() ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m[mt] - mp[mt]);
-        l[mt] *= al;
-        part[mt] *= al;
-        m[mt] = mn;
-      }
-      float e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], c, -mp[mt]));
-      part[mt] += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
     }
+    bool none = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) none |= mp[mt] == -__builtin_inff();
+    if (__ballot(none) != 0) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        if (mp[mt] == -__builtin_inff()) mp[mt] = max8(s[mt][0], s[mt][1]) * c;
+    }
+  };
+  auto weigh = [&](const f32x4 (&s)[2], float ref) INLINE {
+    float e[8];
+    const float z = ref == -__builtin_inff() ? 0.0f : ref;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j >> 2][j & 3], c, -z));
+    return ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+  };
+  // The sums of a block, taken again against a new reference where they ran
+  // past 2^64 (the old sum moves to it).
+  auto add = [&](const f32x4 (&s)[MT][2], float (&t)[MT]) INLINE {
+    bool over = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) over |= t[mt] > 0x1p64f;
+    if (__ballot(over) != 0) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+        if (t[mt] > 0x1p64f) {
+          const float mn = fmaxf(mp[mt], max8(s[mt][0], s[mt][1]) * c);
+          const float al = __builtin_amdgcn_exp2f(mp[mt] - mn);
+          l[mt] *= al;
+          acc[mt] *= al;
+          mp[mt] = mn;
+          t[mt] = weigh(s[mt], mn);
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) acc[mt] += t[mt];
   };
   auto flush = [&]() INLINE {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      l[mt] += part[mt];
-      part[mt] = 0.0f;
+      l[mt] += acc[mt];
+      acc[mt] = 0.0f;
     }
   };
-  const int first = j_begin + KB * w;
-  const int nblk = j_end > first ? (j_end - first + 4 * KB - 1) / (4 * KB) : 0;
-  auto jb = [&](int i) { return first + 4 * KB * min(i, nblk - 1); };
-  if (nblk > 0) {
-    u32x4 ka[2][NKS], kb[2][NKS];
-    load_block(jb(0), ka);
-    for (int i = 0; i < nblk; i += 2) {
-      load_block(jb(i + 1), kb);
-      block(jb(i), ka);
-      if (i + 1 >= nblk) break;
-      load_block(jb(i + 2), ka);
-      block(jb(i + 1), kb);
-      if ((i & 14) == 14) flush();
+  auto sums = [&](const f32x4 (&s)[MT][2], float (&t)[MT]) INLINE {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) t[mt] = weigh(s[mt], mp[mt]);
+  };
+
+  u32x4 kr[Part::NL];
+  auto key_rsrc = [&](int j0, int rows) INLINE {
+    return rows_rsrc(kbase + int64_t(min(j0, P.s_k - 1)) * P.k_ss, P.s_k - j0, rows, kss, D);
+  };
+  f32x4 sa[MT][2], sb[MT][2];
+  float t[MT];
+  if constexpr (SHARE) {
+    // Tile t in stage t & 1.  Step 2 t: exponentials of its first 32 keys,
+    // scores of its second 32; then tile t + 1 is stored.  Step 2 t + 1:
+    // exponentials of the second 32, scores of tile t + 1's first 32.
+    const bool active = row0 < P.s_q;
+    auto load = [&](int tile) INLINE {
+      part.load_at(key_rsrc(j_begin + kTileRows * tile + 16 * w, 16), 0, kr);
+    };
+    if (n_tiles > 0) {
+      load(0);
+      __syncthreads();  // the held rows have left LDS
+      part.store(lds + w * Part::BYTES, kr);
+      load(1);
+      __syncthreads();
+      if (active) scores(lds, sa);
     }
-    flush();
+    for (int tile = 0; tile < n_tiles; ++tile) {
+      const unsigned char* cur = lds + (tile & 1) * Shape::STAGE;
+      unsigned char* nxt = lds + ((tile + 1) & 1) * Shape::STAGE;
+      const int j0 = j_begin + kTileRows * tile;
+      if (active) {
+        prepare(j0, sa);
+        scores(cur + 2 * Part::BYTES, sb);
+        sums(sa, t);
+        add(sa, t);
+      }
+      part.store(nxt + w * Part::BYTES, kr);
+      load(tile + 2);
+      __syncthreads();
+      if (active) {
+        prepare(j0 + 32, sb);
+        scores(nxt, sa);
+        sums(sb, t);
+        add(sb, t);
+      }
+      if ((tile & 7) == 7) flush();
+    }
+  } else {
+    // wave w takes 32-key blocks w, w + 4, ... through its own half stage
+    unsigned char* mine = lds + w * 2 * Part::BYTES;
+    u32x4 kr2[Part::NL];
+    auto load = [&](int j0) INLINE {
+      part.load_at(key_rsrc(j0, 16), 0, kr);
+      part.load_at(key_rsrc(j0 + 16, 16), 0, kr2);
+    };
+    const int first = j_begin + 32 * w;
+    __syncthreads();  // the held rows have left LDS
+    load(first);
+    for (int j0 = first, i = 0; j0 < j_end; j0 += 128, ++i) {
+      part.store(mine, kr);
+      part.store(mine + Part::BYTES, kr2);
+      wave_lds_fence();
+      load(j0 + 128);
+      scores(mine, sa);
+      wave_lds_fence();
+      prepare(j0, sa);
+      sums(sa, t);
+      add(sa, t);
+      if ((i & 15) == 15) flush();
+    }
   }
+  flush();
 
   // merge a row's lanes, then the waves
+  float m[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
+    m[mt] = mp[mt];
 #pragma unroll
     for (int off = 16; off <= 32; off <<= 1) {
       const float mo = __shfl_xor(m[mt], off, 64), lo = __shfl_xor(l[mt], off, 64);
@@ -174,19 +282,27 @@ void sums_stats_kernel(const SumsParams P) {
     }
   }
   __syncthreads();
-  if (tid < 16 * MT) {
-    float M = -__builtin_inff(), L = 0.0f;
+  constexpr int ROWS = 16 * MT * (SHARE ? 4 : 1);
+  if (tid < ROWS) {
+    float M, L;
+    if constexpr (SHARE) {
+      M = sm[tid / (16 * MT)][tid % (16 * MT)];
+      L = sl[tid / (16 * MT)][tid % (16 * MT)];
+    } else {
+      M = -__builtin_inff();
+      L = 0.0f;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) M = fmaxf(M, sm[v][tid]);
+      for (int v = 0; v < 4; ++v) M = fmaxf(M, sm[v][tid]);
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
-      if (sm[v][tid] != -__builtin_inff()) L += __builtin_amdgcn_exp2f(sm[v][tid] - M) * sl[v][tid];
-    const int64_t row = int64_t(bh) * P.s_q_pad + row0 + tid;
-    if (row0 + tid < P.s_q_pad) {
+      for (int v = 0; v < 4; ++v)
+        if (sm[v][tid] != -__builtin_inff() || sl[v][tid] != 0.0f)
+          L += __builtin_amdgcn_exp2f(sm[v][tid] - M) * sl[v][tid];
+    }
+    const int64_t row = int64_t(bh) * P.s_q_pad + wg_row0 + tid;
+    if (wg_row0 + tid < P.s_q_pad) {
       if (P.n_split > 1) {
-        float2* part = reinterpret_cast<float2*>(P.part) +
-                       int64_t(split) * P.batch * P.heads * P.s_q_pad;
-        part[row] = make_float2(M, L);
+        float2* o = reinterpret_cast<float2*>(P.part) + int64_t(split) * P.batch * P.heads * P.s_q_pad;
+        o[row] = make_float2(M, L);
       } else {
         P.stat_m[row] = M == -__builtin_inff() ? 0.0f : M;
         P.stat_r[row] = L == 0.0f ? 0.0f : 1.0f / L;
@@ -227,9 +343,14 @@ __global__ __launch_bounds__(256) void sums_merge_kernel(const SumsParams P) {
 template <typename T, int D>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
 void sums_cols_kernel(const SumsParams P) {
-  constexpr int NKS = SumsShape<D>::NKS, NT = SumsShape<D>::TILES;
+  using Shape = SumsShape<D>;
+  using Part = typename Shape::Part;
+  constexpr int NKS = Shape::NKS, NT = Shape::TILES;
   constexpr int TK = 16 * NT;  // keys of a wave
-  __shared__ float red[4][TK];
+  __shared__ __align__(16) unsigned char lds[2 * Shape::STAGE];
+  // m and 1 / l of the tiles' rows: a wave may still weigh a tile's second half
+  // when another stores the tile after next, so three of them
+  __shared__ __align__(16) float stat[3][2][kTileRows];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane >> 4, lc = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // longest items (first keys) first
@@ -239,108 +360,141 @@ void sums_cols_kernel(const SumsParams P) {
   const int rsplit = x % P.n_rsplit;
   const int kt = x / P.n_rsplit;
   const int b = bkv / P.kv_heads, kvh = bkv - b * P.kv_heads;
-  const int j0 = P.wave_keys ? (4 * kt + w) * TK : kt * TK;
+  const int j0 = (4 * kt + w) * TK;
   const int shift = P.s_k - P.s_q;
   const float c = P.scale_log2;
+  const bool active = j0 < P.s_k;
 
-  float acc[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
-  if (j0 < P.s_k) {
-    const uint16_t* kbase = reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + int64_t(kvh) * P.k_sh;
-    u32x4 kb[NT][NKS];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const uint16_t* krow = kbase + int64_t(min(j0 + 16 * t + lc, P.s_k - 1)) * P.k_ss;
-#pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) kb[t][ks] = load16(krow + 32 * ks + 8 * lr);
+  u32x4 kb[NT][NKS];
+  hold_rows<D, NT>(reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + int64_t(kvh) * P.k_sh +
+                       int64_t(min(j0, P.s_k - 1)) * P.k_ss,
+                   P.s_k - j0, P.k_ss, lane, lds + w * Part::BYTES, kb);
+
+  // 64-row tiles from the first row that sees the item's first key (to 16), of
+  // every head of the kv head
+  const int rb = max(0, 4 * kt * TK - shift) / 16 * 16;
+  const int nt = (P.s_q - rb + kTileRows - 1) / kTileRows;
+  const int total = nt * P.group;
+  const int t0 = int(int64_t(total) * rsplit / P.n_rsplit);
+  const int t1 = int(int64_t(total) * (rsplit + 1) / P.n_rsplit);
+
+  const uint32_t qss = uint32_t(P.q_ss) * 2u;
+  const Part part(lane, qss);
+  u32x4 qr[Part::NL];
+  float st;  // lanes 0..15: m of this wave's rows of the tile, 16..31: 1 / l
+  int lg = t0 / nt, lt = t0 - lg * nt;  // head and tile the next load takes
+  auto load = [&]() INLINE {
+    const int h = kvh * P.group + min(lg, P.group - 1), r = rb + kTileRows * lt + 16 * w;
+    const int rc = min(r, P.s_q - 1);
+    part.load_at(rows_rsrc(reinterpret_cast<const uint16_t*>(P.q) + b * P.q_sb + int64_t(h) * P.q_sh +
+                               int64_t(rc) * P.q_ss,
+                           P.s_q - r, 16, qss, D),
+                 0, qr);
+    if (lane < 32) {
+      const float* src = lane < 16 ? P.stat_m : P.stat_r;
+      st = src[(int64_t(b) * P.heads + h) * P.s_q_pad + min(r + lc, P.s_q - 1)];
     }
-    const uint32_t qss = uint32_t(P.q_ss) * 2u;
-    const uint32_t qoff = uint32_t(lc) * qss + 16u * lr;
-    // 16-row blocks from the first row that sees key j0, of every head
-    const int rb0 = max(0, j0 - shift) / 16, nb = P.s_q_pad / 16 - rb0;
-    const int total = nb * P.group;
-    const int t0 = int(int64_t(total) * rsplit / P.n_rsplit);
-    const int t1 = int(int64_t(total) * (rsplit + 1) / P.n_rsplit);
-    const int step = P.wave_keys ? 1 : 4, first = t0 + (P.wave_keys ? 0 : w);
+    if (++lt == nt) {
+      lt = 0;
+      ++lg;
+    }
+  };
+  auto store = [&](int stage, int slot) INLINE {
+    part.store(lds + stage * Shape::STAGE + w * Part::BYTES, qr);
+    if (lane < 32) stat[slot][lane >> 4][16 * w + lc] = st;
+  };
 
-    auto load_block = [&](int t, u32x4 (&qr)[NKS], f32x4& sm, f32x4& sr) INLINE {
-      const int g = t / nb, r0 = 16 * (rb0 + t - g * nb);
-      const int h = kvh * P.group + g;
-      const uint16_t* q0 = reinterpret_cast<const uint16_t*>(P.q) + b * P.q_sb + int64_t(h) * P.q_sh +
-                           int64_t(r0) * P.q_ss;
-      const __amdgpu_buffer_rsrc_t rs = rows_rsrc(q0, P.s_q - r0, 16, qss, D);
+  float acc[NT], sum[NT];
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks)
-        qr[ks] = __builtin_bit_cast(
-            u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, qoff + 64 * ks, 0, 0));
-      const int64_t row = (int64_t(b) * P.heads + h) * P.s_q_pad + r0 + 4 * lr;
-      sm = *reinterpret_cast<const f32x4*>(P.stat_m + row);
-      sr = *reinterpret_cast<const f32x4*>(P.stat_r + row);
-    };
-    float part[NT];
+  for (int n = 0; n < NT; ++n) acc[n] = sum[n] = 0.0f;
+  auto scores = [&](const unsigned char* lp, f32x4 (&s)[NT][2]) INLINE {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) part[t] = 0.0f;
-    auto block = [&](int t, const u32x4 (&qr)[NKS], const f32x4& sm, const f32x4& sr) INLINE {
-      const int row = 16 * (rb0 + t % nb);
-      const bool edge = shift + row < j0 + TK - 1 || row + 16 > P.s_q;
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        f32x4 s = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int n = 0; n < NT; ++n) s[n][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks) s = mfma_qk<T>(qr[ks], kb[n][ks], s);
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4 a = Part::operand(lp + u * Part::BYTES, 0, lc, lr, ks);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][u] = mfma_qk<T>(a, kb[n][ks], s[n][u]);
+      }
+    }
+  };
+  // 32 rows from row r on, whose (m, 1 / l) are sp[.] and sp[kTileRows + .]
+  auto weigh = [&](int r, const float* sp, const f32x4 (&s)[NT][2]) INLINE {
+    const bool edge = shift + r < j0 + TK - 1 || r + 32 > P.s_q;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const f32x4 m = *reinterpret_cast<const f32x4*>(sp + 16 * u + 4 * lr);
+      const f32x4 inv = *reinterpret_cast<const f32x4*>(sp + kTileRows + 16 * u + 4 * lr);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -sm[i])), r = sr[i];
-          const int ri = row + 4 * lr + i;
-          if (edge && (shift + ri < j0 + 16 * n + lc || ri >= P.s_q)) e = r = 0.0f;
-          part[n] = __builtin_fmaf(e, r, part[n]);
+          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][u][i], c, -m[i])), f = inv[i];
+          const int ri = r + 16 * u + 4 * lr + i;
+          if (edge && (shift + ri < j0 + 16 * n + lc || ri >= P.s_q)) e = f = 0.0f;
+          acc[n] = __builtin_fmaf(e, f, acc[n]);
         }
-      }
-    };
-    auto flush = [&]() INLINE {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        acc[n] += part[n];
-        part[n] = 0.0f;
-      }
-    };
-    const int nblk = t1 > first ? (t1 - first + step - 1) / step : 0;
-    auto tb = [&](int i) { return first + step * min(i, nblk - 1); };
-    if (nblk > 0) {
-      u32x4 qa[NKS], qc[NKS];
-      f32x4 ma, ra, mc, rc;
-      load_block(tb(0), qa, ma, ra);
-      for (int i = 0; i < nblk; i += 2) {
-        load_block(tb(i + 1), qc, mc, rc);
-        block(tb(i), qa, ma, ra);
-        if (i + 1 >= nblk) break;
-        load_block(tb(i + 2), qa, ma, ra);
-        block(tb(i + 1), qc, mc, rc);
-        if ((i & 14) == 14) flush();
-      }
-      flush();
     }
+  };
+  auto flush = [&]() INLINE {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      acc[n] += __shfl_xor(acc[n], 16, 64);
-      acc[n] += __shfl_xor(acc[n], 32, 64);
+      sum[n] += acc[n];
+      acc[n] = 0.0f;
     }
+  };
+
+  f32x4 sa[NT][2], sb[NT][2];
+  if (t1 > t0) {
+    load();
+    __syncthreads();  // the held keys have left LDS
+    store(0, 0);
+    load();
+    __syncthreads();
+    if (active) scores(lds, sa);
   }
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-    if (lr == 0) red[w][16 * n + lc] = acc[n];
-  __syncthreads();
-  const int nk = P.wave_keys ? 4 * TK : TK, jt = kt * nk;
-  for (int y = tid; y < nk && jt + y < P.s_k; y += 256) {
-    const float r = P.wave_keys ? red[y / TK][y % TK]
-                                : (red[0][y] + red[1][y]) + (red[2][y] + red[3][y]);
-    if (P.n_rsplit > 1) {
-      P.col_part[(int64_t(rsplit) * P.batch * P.kv_heads + bkv) * P.s_k + jt + y] = r;
-    } else {
-      float* o = P.sums + b * P.s_sb + kvh * P.s_sh + jt + y;
-      *o = P.add ? *o + r : r;
+  int ct = t0 % nt, slot = 0;
+  for (int t = t0; t < t1; ++t) {
+    // as the stats steps: stage (t - t0) & 1
+    const int cs = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1;
+    const float* sp = stat[slot][0];
+    const int r = rb + kTileRows * ct;
+    if (++ct == nt) ct = 0;
+    // rows before this wave's first key see none of its keys
+    const bool see0 = active && shift + r + 31 >= j0, see1 = active && shift + r + 63 >= j0;
+    if (active) {
+      scores(lds + cs * Shape::STAGE + 2 * Part::BYTES, sb);
+      if (see0) weigh(r, sp, sa);
     }
+    store(1 - cs, next);
+    load();
+    __syncthreads();
+    if (active) {
+      scores(lds + (1 - cs) * Shape::STAGE, sa);
+      if (see1) weigh(r + 32, sp + 32, sb);
+    }
+    slot = next;
+    if ((t & 7) == 7) flush();
+  }
+  flush();
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    sum[n] += __shfl_xor(sum[n], 16, 64);
+    sum[n] += __shfl_xor(sum[n], 32, 64);
+  }
+  // lane: key 16 lr + lc of the wave's (lr < NT)
+  float r = sum[0];
+#pragma unroll
+  for (int n = 1; n < NT; ++n) r = lr == n ? sum[n] : r;
+  const int j = j0 + 16 * lr + lc;
+  if (lr >= NT || j >= P.s_k) return;
+  if (P.n_rsplit > 1) {
+    P.col_part[(int64_t(rsplit) * P.batch * P.kv_heads + bkv) * P.s_k + j] = r;
+  } else {
+    float* o = P.sums + b * P.s_sb + kvh * P.s_sh + j;
+    *o = P.add ? *o + r : r;
   }
 }
 
@@ -361,10 +515,12 @@ hipError_t launch_sums_d(const SumsParams& p, hipStream_t st) {
   constexpr int NT = SumsShape<D>::TILES;
   const int64_t bh = int64_t(p.batch) * p.heads;
   const dim3 ga(uint32_t(bh * p.n_rt * p.n_split));
-  if (p.mt == 1)
-    hipLaunchKernelGGL((sums_stats_kernel<T, D, 1>), ga, dim3(256), 0, st, p);
+  if (p.share)
+    hipLaunchKernelGGL((sums_stats_kernel<T, D, NT, true>), ga, dim3(256), 0, st, p);
+  else if (p.stat_rows == 16)
+    hipLaunchKernelGGL((sums_stats_kernel<T, D, 1, false>), ga, dim3(256), 0, st, p);
   else
-    hipLaunchKernelGGL((sums_stats_kernel<T, D, NT>), ga, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((sums_stats_kernel<T, D, NT, false>), ga, dim3(256), 0, st, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   if (p.n_split > 1) {
