@@ -14,8 +14,7 @@
 //     i.  Each lane sums its keys' weights in registers.
 // The walked rows go through LDS, 64 a tile, for the four waves of a workgroup
 // (256 rows or keys); with at most 64 rows in all the waves of a stats item
-// take different keys instead.  The scores of the next 32 rows are multiplied
-// while the exponentials of the last 32 are taken.
+// take different keys instead.
 // Bound by the exponentials, two for each visible pair (a quarter-rate
 // instruction), with a fused multiply-add and an add beside each.
 // Sums are fp32 in two levels, in a fixed order.
@@ -73,7 +72,7 @@ __device__ inline void hold_rows(const uint16_t* p, int left, int64_t stride, in
 // SHARE: four waves of 16 MT rows each against the same keys; otherwise one set
 // of rows, the waves on different keys.
 template <typename T, int D, int MT, bool SHARE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : SHARE && D <= 128 ? 3 : 2)))
 void sums_stats_kernel(const SumsParams P) {
   using Shape = SumsShape<D>;
   using Part = typename Shape::Part;
@@ -130,10 +129,12 @@ void sums_stats_kernel(const SumsParams P) {
       }
     }
   };
+  auto edge = [&](int j0) INLINE { return j0 + 31 > shift + row0 || j0 + 32 > j_end; };
+  bool started = false;  // every lane has a reference
   // Hides what a row does not see, and starts the reference of a lane that has
   // none yet.
   auto prepare = [&](int j0, f32x4 (&s)[MT][2]) INLINE {
-    if (j0 + 31 > shift + row0 || j0 + 32 > j_end) {
+    if (edge(j0)) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const int last = min(shift + row0 + 16 * mt + lc, j_end - 1);
@@ -147,7 +148,8 @@ void sums_stats_kernel(const SumsParams P) {
     bool none = false;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) none |= mp[mt] == -__builtin_inff();
-    if (__ballot(none) != 0) {
+    started = __ballot(none) == 0;
+    if (!started) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
         if (mp[mt] == -__builtin_inff()) mp[mt] = max8(s[mt][0], s[mt][1]) * c;
@@ -189,21 +191,22 @@ void sums_stats_kernel(const SumsParams P) {
       acc[mt] = 0.0f;
     }
   };
-  auto sums = [&](const f32x4 (&s)[MT][2], float (&t)[MT]) INLINE {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) t[mt] = weigh(s[mt], mp[mt]);
-  };
 
   u32x4 kr[Part::NL];
   auto key_rsrc = [&](int j0, int rows) INLINE {
     return rows_rsrc(kbase + int64_t(min(j0, P.s_k - 1)) * P.k_ss, P.s_k - j0, rows, kss, D);
   };
-  f32x4 sa[MT][2], sb[MT][2];
-  float t[MT];
+  auto block = [&](int j0, const unsigned char* lp) INLINE {
+    f32x4 s[MT][2];
+    float t[MT];
+    scores(lp, s);
+    if (!started || edge(j0)) prepare(j0, s);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) t[mt] = weigh(s[mt], mp[mt]);
+    add(s, t);
+  };
   if constexpr (SHARE) {
-    // Tile t in stage t & 1.  Step 2 t: exponentials of its first 32 keys,
-    // scores of its second 32; then tile t + 1 is stored.  Step 2 t + 1:
-    // exponentials of the second 32, scores of tile t + 1's first 32.
+    // tile t in stage t & 1, the next one on its way through registers
     const bool active = row0 < P.s_q;
     auto load = [&](int tile) INLINE {
       part.load_at(key_rsrc(j_begin + kTileRows * tile + 16 * w, 16), 0, kr);
@@ -214,27 +217,17 @@ void sums_stats_kernel(const SumsParams P) {
       part.store(lds + w * Part::BYTES, kr);
       load(1);
       __syncthreads();
-      if (active) scores(lds, sa);
     }
     for (int tile = 0; tile < n_tiles; ++tile) {
       const unsigned char* cur = lds + (tile & 1) * Shape::STAGE;
       unsigned char* nxt = lds + ((tile + 1) & 1) * Shape::STAGE;
       const int j0 = j_begin + kTileRows * tile;
-      if (active) {
-        prepare(j0, sa);
-        scores(cur + 2 * Part::BYTES, sb);
-        sums(sa, t);
-        add(sa, t);
-      }
+      if (active)
+        for (int half = 0; half < 2; ++half)
+          block(j0 + 32 * half, cur + 2 * half * Part::BYTES);
       part.store(nxt + w * Part::BYTES, kr);
       load(tile + 2);
       __syncthreads();
-      if (active) {
-        prepare(j0 + 32, sb);
-        scores(nxt, sa);
-        sums(sb, t);
-        add(sb, t);
-      }
       if ((tile & 7) == 7) flush();
     }
   } else {
@@ -253,11 +246,8 @@ void sums_stats_kernel(const SumsParams P) {
       part.store(mine + Part::BYTES, kr2);
       wave_lds_fence();
       load(j0 + 128);
-      scores(mine, sa);
+      block(j0, mine);
       wave_lds_fence();
-      prepare(j0, sa);
-      sums(sa, t);
-      add(sa, t);
       if ((i & 15) == 15) flush();
     }
   }
@@ -341,7 +331,7 @@ __global__ __launch_bounds__(256) void sums_merge_kernel(const SumsParams P) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : D > 128 ? 2 : 3)))
 void sums_cols_kernel(const SumsParams P) {
   using Shape = SumsShape<D>;
   using Part = typename Shape::Part;
@@ -421,8 +411,7 @@ void sums_cols_kernel(const SumsParams P) {
     }
   };
   // 32 rows from row r on, whose (m, 1 / l) are sp[.] and sp[kTileRows + .]
-  auto weigh = [&](int r, const float* sp, const f32x4 (&s)[NT][2]) INLINE {
-    const bool edge = shift + r < j0 + TK - 1 || r + 32 > P.s_q;
+  auto weigh = [&](int r, bool edge, const float* sp, const f32x4 (&s)[NT][2]) INLINE {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const f32x4 m = *reinterpret_cast<const f32x4*>(sp + 16 * u + 4 * lr);
@@ -446,35 +435,34 @@ void sums_cols_kernel(const SumsParams P) {
     }
   };
 
-  f32x4 sa[NT][2], sb[NT][2];
   if (t1 > t0) {
     load();
     __syncthreads();  // the held keys have left LDS
     store(0, 0);
     load();
     __syncthreads();
-    if (active) scores(lds, sa);
   }
   int ct = t0 % nt, slot = 0;
   for (int t = t0; t < t1; ++t) {
-    // as the stats steps: stage (t - t0) & 1
     const int cs = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1;
     const float* sp = stat[slot][0];
     const int r = rb + kTileRows * ct;
     if (++ct == nt) ct = 0;
-    // rows before this wave's first key see none of its keys
-    const bool see0 = active && shift + r + 31 >= j0, see1 = active && shift + r + 63 >= j0;
-    if (active) {
-      scores(lds + cs * Shape::STAGE + 2 * Part::BYTES, sb);
-      if (see0) weigh(r, sp, sa);
-    }
+    if (active)
+      for (int half = 0; half < 2; ++half) {
+        const int rh = r + 32 * half;
+        const bool edge = shift + rh < j0 + TK - 1 || rh + 32 > P.s_q;
+        if (edge && shift + rh + 31 < j0) continue;  // before this wave's first key
+        f32x4 s[NT][2];
+        scores(lds + cs * Shape::STAGE + 2 * half * Part::BYTES, s);
+        if (edge)
+          weigh(rh, true, sp + 32 * half, s);
+        else
+          weigh(rh, false, sp + 32 * half, s);
+      }
     store(1 - cs, next);
     load();
     __syncthreads();
-    if (active) {
-      scores(lds + (1 - cs) * Shape::STAGE, sa);
-      if (see1) weigh(r + 32, sp + 32, sb);
-    }
     slot = next;
     if ((t & 7) == 7) flush();
   }
