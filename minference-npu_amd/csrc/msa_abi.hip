@@ -1319,29 +1319,37 @@ int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const
   rp.n_rto = int(cdiv(rows, rp.own_rows));
   rows_split(Sp, std::min<int64_t>(cdiv(Sp, 256), cdiv(512, rp.n_rt * Hkv)),
              kp ? rows_max_chunk(kp, vp) : 128, rp.n_sp, rp.chunk_p);
-  rows_split(Sc, std::min<int64_t>(cdiv(Sc, 256), cdiv(2048, rp.n_rto * B * Hkv)),
-             rows_max_chunk(k, v), rp.n_so, rp.chunk_o);
-  if (rp.n_sp + rp.n_so > kRowsMaxSplit) return MSA_E_SEQ;
-  const int64_t np = cdiv(Hkv * rp.n_sp, 8) * 8 * rp.n_rt, no = B * Hkv * rp.n_so * rp.n_rto;
-  if (np + no >= (int64_t(1) << 31)) return MSA_E_HEADS;
+  // own caches: one item per workgroup slot (two a CU), more where a descriptor
+  // could not cover an item's keys
+  const int64_t triples = B * Hkv * rp.n_rto, units = triples * cdiv(Sc, 128);
+  const int64_t most = rows_max_chunk(k, v) / 128;  // units of an item
+  rp.min_units = int(std::min<int64_t>(2, most));
+  const int64_t n_own = std::min(cdiv(units, rp.min_units), std::max<int64_t>(512, cdiv(units, most)));
+  const int64_t row_splits = std::min(n_own, cdiv(cdiv(Sc, 128), rp.min_units) + 1);
+  if (rp.n_sp + row_splits > kRowsMaxSplit) return MSA_E_SEQ;
+  const int64_t np = cdiv(Hkv * rp.n_sp, 8) * 8 * rp.n_rt;
+  if (np + n_own >= (int64_t(1) << 31) || units >= (int64_t(1) << 30)) return MSA_E_HEADS;
+  rp.n_own = int(n_own);
   rp.n_prefix_items = int(np);
-  rp.n_items = int(np + no);
+  rp.n_items = int(np + rp.n_own);
+  rp.raw_row = cdiv(Sc, 32) * 32;
   rp.own_row0 = Hkv * rp.n_sp * R;
   return MSA_OK;
 }
 
-// Workspace: part, then ml, then (decode_accumulate) the raw scores.
+// Workspace: part, ml, the own caches' plan, then (decode_accumulate) the raw scores.
 struct RowsLayout {
-  size_t ml, raw, total;
+  size_t ml, plan, raw, total;
 };
 RowsLayout rows_layout(const RowsParams& rp, int64_t D, bool raw) {
-  const size_t n = size_t(rp.own_row0 + int64_t(rp.batch) * rp.heads * rp.s_q * rp.n_so);
+  const int64_t own = rp.n_own + int64_t(rp.batch) * rp.kv_heads * rp.n_rto;
+  const size_t n = size_t(rp.own_row0 + own * rp.own_rows);
   const auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   RowsLayout l;
   l.ml = up(n * size_t(D) * 4);
-  l.raw = l.ml + up(n * 8);
-  l.total = l.raw + (raw ? up(size_t(rp.batch) * rp.heads * rp.s_c * 4) : 0);
-  if (l.total == 0) l.total = 256;
+  l.plan = l.ml + up(n * 8);
+  l.raw = l.plan + up(size_t(rp.batch + 1) * 4);
+  l.total = l.raw + (raw ? up(size_t(rp.batch) * rp.heads * rp.raw_row * 4) : 0);
   return l;
 }
 
@@ -1397,6 +1405,7 @@ void rows_fill(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* k, const
   rp.scale_log2 = float(double(scale) * 1.4426950408889634);
   rp.part = ws_at<float>(workspace, 0);
   rp.ml = ws_at<float>(workspace, l.ml);
+  rp.plan = ws_at<int32_t>(workspace, l.plan);
   rp.raw = ws_at<float>(workspace, l.raw);
 }
 
@@ -1515,9 +1524,9 @@ int sums_plan(SumsParams& sp, SumsLayout& l, const msa_tensor4* q, const msa_ten
   sp.n_rt = int(cdiv(Sq, sp.stat_rows));
   // stats: key splits where there are few items
   const int64_t items = BH * sp.n_rt;
-  const int64_t want = std::min<int64_t>(cdiv(Sk, 512), cdiv(1024, items));
+  const int64_t want = std::min<int64_t>(cdiv(Sk, 512), cdiv(2304, items));
   sp.chunk = int(cdiv(cdiv(Sk, want), 128) * 128);
-  sp.n_split = items >= 512 ? 1 : int(cdiv(Sk, sp.chunk));
+  sp.n_split = items >= 1536 ? 1 : int(cdiv(Sk, sp.chunk));
   if (sp.n_split == 1) sp.chunk = int(cdiv(Sk, 128) * 128);
   // columns: row splits where there are few items, of at least 8 tiles of 64 rows
   sp.n_kt = int(cdiv(Sk, 64 * tiles));

@@ -240,14 +240,16 @@ struct RowsParams {
   int prefix_form, own_form;  // of the items (rows_forms), and their rows
   int prefix_rows, own_rows;
   int n_rt, n_sp, chunk_p;   // prefix: row tiles, key splits, keys of a split
-  int n_rto, n_so, chunk_o;  // own caches: the same per (sequence, kv head)
+  int n_rto, n_own, min_units;  // own caches: row tiles, items, least units of 128 keys of one
   int n_prefix_items, n_items;  // prefix: (kv head, split) pairs to a multiple of 8
   float scale_log2;          // softmax scale * log2(e)
   float* part;               // partial O, [row][D]: prefix [kv_heads][n_sp][batch * rows],
-                             // from own_row0 on own [batch][kv_heads][n_so][rows]
+                             // from own_row0 on [n_own + batch * kv_heads * n_rto][own_rows]
   float* ml;                 // (m, l) of each row of part
   int64_t own_row0;
-  float* raw;                // decode_accumulate: raw scores [batch][heads][s_c]
+  int32_t* plan;             // [1 + batch]: the first launch's split of the own caches
+  float* raw;                // decode_accumulate: raw scores [batch][heads][raw_row]
+  int64_t raw_row;
   const float* w_in;         // scores before and after, [batch][kv_heads][s_c]
   float* w_out;
   int64_t wi_sb, wi_sh, wo_sb, wo_sh;

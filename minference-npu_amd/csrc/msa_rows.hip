@@ -27,7 +27,8 @@
 // rows; both are read once per item.  Softmax statistics
 // and O are fp32; a row's running max moves only when a block exceeds it by
 // 2^kSlack.  P is rounded to the inputs' type twice, P and what that rounding
-// left, so the product's error stays below the output's own rounding.
+// left, so the product's error stays below the output's own rounding (kTwoParts
+// names the exception).
 // Each item leaves O and (m, l) of its rows in the workspace; the combine
 // kernel merges the items of a row.
 
@@ -289,14 +290,10 @@ __device__ void rows_item(const RowsParams& P, const Item& it, Shared& sh) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       f32x4(&s)[2] = st[mt];
-      if (SCORES && lc < it.n_rows) {  // MT == 1
+      if (SCORES && lc < it.n_rows) {  // MT == 1; rows of raw end with a multiple of 32 keys
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = j0 + 16 * u + 4 * lr + i;
-            if (j < it.n_keys) it.raw[lc * it.raw_row + j] = s[u][i];
-          }
+          *reinterpret_cast<f32x4*>(it.raw + lc * it.raw_row + j0 + 16 * u + 4 * lr) = s[u];
       }
       if (edge) {
 #pragma unroll
@@ -481,6 +478,13 @@ __device__ void rows_item(const RowsParams& P, const Item& it, Shared& sh) {
   }
 }
 
+// Whether a kTile item holds P in two parts.  In bf16 one part (8 bits) would
+// round as coarsely as the output; in fp16 (11 bits, what the prefill kernels
+// round P to) one is enough, and a third of the PV work: 128 sequences on 8 x
+// 32768 x 128 take 128 us with two parts, 108 with one.
+template <typename T>
+constexpr bool kTwoParts = T::id == Bf16::id;
+
 // kTile: 64 keys of K and V at a time in LDS for the four waves, the next tile
 // on its way through registers.  V operands are transposing LDS reads: a group of
 // 16 lanes takes 4 keys of 16 dims, which is the key order of P.
@@ -600,8 +604,10 @@ __device__ void rows_tile_item(const RowsParams& P, const Item& it, Shared& sh) 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         ph[mt][j] = pack2<T>(p[2 * j], p[2 * j + 1]);
-        pl[mt][j] = pack2<T>(__builtin_fmaf(lo_of<T>(ph[mt][j]), -1.0f, p[2 * j]),
-                             __builtin_fmaf(hi_of<T>(ph[mt][j]), -1.0f, p[2 * j + 1]));
+        pl[mt][j] = 0;
+        if constexpr (kTwoParts<T>)
+          pl[mt][j] = pack2<T>(__builtin_fmaf(lo_of<T>(ph[mt][j]), -1.0f, p[2 * j]),
+                               __builtin_fmaf(hi_of<T>(ph[mt][j]), -1.0f, p[2 * j + 1]));
       }
     }
     const unsigned char* vl = stage + 4 * Part::BYTES + (32 * h + 4 * lr + (lc >> 2)) * VS + 8 * (lc & 3);
@@ -626,7 +632,7 @@ __device__ void rows_tile_item(const RowsParams& P, const Item& it, Shared& sh) 
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         o[mt][n] = mfma_qk<T>(a, ph[mt], o[mt][n]);
-        o[mt][n] = mfma_qk<T>(a, pl[mt], o[mt][n]);
+        if constexpr (kTwoParts<T>) o[mt][n] = mfma_qk<T>(a, pl[mt], o[mt][n]);
       }
     }
   };
@@ -665,6 +671,70 @@ __device__ void rows_tile_item(const RowsParams& P, const Item& it, Shared& sh) 
 
 __device__ inline int clamped_len(const RowsParams& P, int b) {
   return P.lens ? max(0, min(P.lens[b], P.s_c)) : P.s_c;
+}
+
+constexpr int kUnit = 128;  // keys: one round of the four waves
+
+struct OwnPlan {
+  int total;  // units of all own caches
+  int per;    // units of an item
+};
+
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Units of the sequences before each lane's, of b0 .. b0 + 63, and of all of these.
+__device__ inline int own_scan(const RowsParams& P, int b0, int& chunk) {
+  const int lane = threadIdx.x & 63, b = b0 + lane;
+  const int mine = b < P.batch ? (clamped_len(P, b) + kUnit - 1) / kUnit * P.kv_heads * P.n_rto : 0;
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += y;
+  }
+  chunk = __builtin_amdgcn_readlane(incl, 63);
+  return incl - mine;
+}
+
+// The plan of a call; `write`: leaves it for the second launch, plan[0] = per,
+// plan[1 + b] = units before sequence b.
+__device__ inline OwnPlan own_plan(const RowsParams& P, bool write) {
+  OwnPlan p;
+  p.total = 0;
+  for (int b0 = 0; b0 < P.batch; b0 += 64) {
+    int chunk;
+    const int before = own_scan(P, b0, chunk);
+    if (write && threadIdx.x < 64 && b0 + int(threadIdx.x) < P.batch)
+      P.plan[1 + b0 + threadIdx.x] = p.total + before;
+    p.total += chunk;
+  }
+  p.per = uniform(max(P.min_units, (p.total + P.n_own - 1) / P.n_own));
+  if (write && threadIdx.x == 0) P.plan[0] = p.per;
+  return p;
+}
+
+// The sequence that unit u belongs to, and the units before it.
+__device__ inline int own_find(const RowsParams& P, int u, int& before) {
+  int base = 0;
+  for (int b0 = 0;; b0 += 64) {
+    int chunk;
+    const int mine = base + own_scan(P, b0, chunk);
+    if (u < base + chunk || b0 + 64 >= P.batch) {
+      // the last sequence that starts at or before u is not empty: the next
+      // one starts behind u
+      const uint64_t at = __ballot(mine <= u && b0 + int(threadIdx.x & 63) < P.batch);
+      const int last = 63 - __builtin_clzll(at);
+      before = __builtin_amdgcn_readlane(mine, last);
+      return b0 + last;
+    }
+    base += chunk;
+  }
+}
+
+// First row in part / ml of what item x leaves of triple t (kv head, row tile)
+// of sequence b: items and triples are in one order, so x + their number differ.
+__device__ inline int64_t own_part_row(const RowsParams& P, int64_t x, int b, int t) {
+  return P.own_row0 + (x + int64_t(b) * P.kv_heads * P.n_rto + t) * P.own_rows;
 }
 
 template <typename T, int D, int FORM, bool CAUSAL, bool SCORES, typename Shared>
@@ -709,30 +779,48 @@ void rows_kernel(const RowsParams P) {
     if constexpr (PF > 0) run_item<T, D, PF, false, false>(P, it, sh);
     return;
   }
+  // Own caches: the units of 128 keys of all (sequence, kv head, row tile)
+  // triples in a row, cut into equal ranges of P.n_own items, so lengths, known
+  // on the device only, do not leave some workgroups with more than others.
   x -= P.n_prefix_items;
-  const int rt = x % P.n_rto;
-  x /= P.n_rto;
-  const int split = x % P.n_so;
-  x /= P.n_so;
-  it.kvh = x % P.kv_heads;
-  const int b = x / P.kv_heads;
-  const int j0 = split * P.chunk_o;
-  const int len = clamped_len(P, b);
-  it.k = reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + it.kvh * P.k_sh + int64_t(j0) * P.k_ss;
-  it.v = reinterpret_cast<const uint16_t*>(P.v) + b * P.v_sb + it.kvh * P.v_sh + int64_t(j0) * P.v_ss;
-  it.kss = uint32_t(P.k_ss) * 2u;
-  it.vss = uint32_t(P.v_ss) * 2u;
-  it.n_keys = min(P.chunk_o, len - j0);
-  it.limit = len - P.s_q - j0;
-  const int r0 = rt * form_rows(OF);
-  it.row0 = b * it.seq_rows + r0;
-  it.n_rows = min(form_rows(OF), it.seq_rows - r0);
-  it.part_row = P.own_row0 + (int64_t(b * P.kv_heads + it.kvh) * P.n_so + split) * it.seq_rows + r0;
-  if constexpr (SCORES) {  // s_q == 1: rows are the heads of the group
-    it.raw_row = P.s_c;
-    it.raw = P.raw + (int64_t(b) * P.heads + it.kvh * P.group + r0) * P.s_c + j0;
+  const OwnPlan plan = own_plan(P, x == 0);
+  const int per_seq = P.kv_heads * P.n_rto;
+  int u = x * plan.per;
+  const int u_end = min(u + plan.per, plan.total);
+  if (u >= u_end) return;
+  int before;
+  int b = own_find(P, u, before);
+  bool first = true;
+  while (u < u_end) {
+    const int len = uniform(clamped_len(P, b)), n = (len + kUnit - 1) / kUnit;
+    if (u >= before + n * per_seq) {  // sequence b ends here
+      before += n * per_seq;
+      ++b;
+      continue;
+    }
+    const int t = uniform((u - before) / n), k0 = u - before - t * n;
+    const int n_here = min(n - k0, u_end - u);
+    it.kvh = uniform(t / P.n_rto);
+    const int r0 = (t - it.kvh * P.n_rto) * form_rows(OF);
+    const int j0 = k0 * kUnit;
+    it.k = reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + it.kvh * P.k_sh + int64_t(j0) * P.k_ss;
+    it.v = reinterpret_cast<const uint16_t*>(P.v) + b * P.v_sb + it.kvh * P.v_sh + int64_t(j0) * P.v_ss;
+    it.kss = uint32_t(P.k_ss) * 2u;
+    it.vss = uint32_t(P.v_ss) * 2u;
+    it.n_keys = min(n_here * kUnit, len - j0);
+    it.limit = len - P.s_q - j0;
+    it.row0 = b * it.seq_rows + r0;
+    it.n_rows = min(form_rows(OF), it.seq_rows - r0);
+    it.part_row = own_part_row(P, x, b, t);
+    if constexpr (SCORES) {  // s_q == 1: rows are the heads of the group
+      it.raw_row = P.raw_row;
+      it.raw = P.raw + (int64_t(b) * P.heads + it.kvh * P.group + r0) * P.raw_row + j0;
+    }
+    if (!first) __syncthreads();  // LDS of the range before
+    first = false;
+    run_item<T, D, OF, CAUSAL, SCORES>(P, it, sh);
+    u += n_here;
   }
-  run_item<T, D, OF, CAUSAL, SCORES>(P, it, sh);
 }
 
 template <typename T, bool OUT_F32>
@@ -744,14 +832,31 @@ __device__ inline void store_one(void* o, int64_t off, float r) {
   }
 }
 
-// Place in part / ml of split s of row rr of (sequence b, kv head kvh): the
-// prefix splits first, then the own cache's.
-__device__ inline int64_t part_row_of(const RowsParams& P, int b, int kvh, int rr, int s) {
-  const int seq_rows = P.group * P.s_q;
-  if (s < P.n_sp)
-    return (int64_t(kvh) * P.n_sp + s) * P.batch * seq_rows + int64_t(b) * seq_rows + rr;
-  return P.own_row0 + (int64_t(b * P.kv_heads + kvh) * P.n_so + (s - P.n_sp)) * seq_rows + rr;
-}
+// Where the splits of row rr of (sequence b, kv head kvh) lie in part / ml:
+// n_sp of the prefix, then n - n_sp of its own cache.
+struct RowSplits {
+  int n, n_sp;
+  int64_t prefix, prefix_step, own, own_step;
+  __device__ RowSplits(const RowsParams& P, int b, int kvh, int rr) {
+    const int seq_rows = P.group * P.s_q;
+    n = n_sp = P.n_sp;
+    prefix_step = int64_t(P.batch) * seq_rows;
+    prefix = int64_t(kvh) * P.n_sp * prefix_step + int64_t(b) * seq_rows + rr;
+    own = 0;
+    own_step = P.own_rows;
+    const int units = P.n_own > 0 ? (clamped_len(P, b) + kUnit - 1) / kUnit : 0;
+    if (units > 0) {
+      const int rt = rr / P.own_rows, t = kvh * P.n_rto + rt;
+      const int per = P.plan[0], u0 = P.plan[1 + b] + t * units;
+      const int x0 = u0 / per, x1 = (u0 + units - 1) / per;
+      n += x1 - x0 + 1;
+      own = own_part_row(P, x0, b, t) + rr - rt * P.own_rows;
+    }
+  }
+  __device__ int64_t at(int s) const {
+    return s < n_sp ? prefix + s * prefix_step : own + (s - n_sp) * own_step;
+  }
+};
 
 // Output row rr of (b, kvh): O = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s
 // over its splits, by one workgroup.  Splits without a score above -inf leave
@@ -764,10 +869,11 @@ __device__ void combine_row(const RowsParams& P, int b, int kvh, int rr) {
   __shared__ float red[8];
   __shared__ __align__(16) float acc_g[G][D];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int ns = P.n_sp + P.n_so;
+  const RowSplits sp(P, b, kvh, rr);
+  const int ns = sp.n;
   float mx = -__builtin_inff();
   for (int s = tid; s < ns; s += 256) {
-    const float ms = P.ml[2 * part_row_of(P, b, kvh, rr, s)];
+    const float ms = P.ml[2 * sp.at(s)];
     fs[s] = ms;
     mx = fmaxf(mx, ms);
   }
@@ -781,7 +887,7 @@ __device__ void combine_row(const RowsParams& P, int b, int kvh, int rr) {
     const float ms = fs[s];
     const float f = ms == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
     fs[s] = f;
-    L += f * P.ml[2 * part_row_of(P, b, kvh, rr, s) + 1];
+    L += f * P.ml[2 * sp.at(s) + 1];
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) L += __shfl_xor(L, off, 64);
@@ -795,7 +901,7 @@ __device__ void combine_row(const RowsParams& P, int b, int kvh, int rr) {
     for (int s = g; s < ns; s += G) {
       const float f = fs[s];
       if (f == 0.0f) continue;
-      const float4 x = *reinterpret_cast<const float4*>(P.part + part_row_of(P, b, kvh, rr, s) * D + 4 * c);
+      const float4 x = *reinterpret_cast<const float4*>(P.part + sp.at(s) * D + 4 * c);
       a0 = __builtin_fmaf(f, x.x, a0);
       a1 = __builtin_fmaf(f, x.y, a1);
       a2 = __builtin_fmaf(f, x.z, a2);
@@ -842,13 +948,14 @@ __global__ __launch_bounds__(256) void rows_weights_kernel(const RowsParams P, i
   if (j0 >= len) return;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   for (int g = w; g < P.group; g += 4) {  // (M, 1 / L) of each head
+    const RowSplits sp(P, b, kvh, g);
     float M = -__builtin_inff();
-    for (int s = lane; s < P.n_so; s += 64) M = fmaxf(M, P.ml[2 * part_row_of(P, b, kvh, g, s)]);
+    for (int s = lane; s < sp.n; s += 64) M = fmaxf(M, P.ml[2 * sp.at(s)]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
     float L = 0.0f;
-    for (int s = lane; s < P.n_so; s += 64) {
-      const int64_t pr = part_row_of(P, b, kvh, g, s);
+    for (int s = lane; s < sp.n; s += 64) {
+      const int64_t pr = sp.at(s);
       const float ms = P.ml[2 * pr];
       if (ms != -__builtin_inff()) L += __builtin_amdgcn_exp2f(ms - M) * P.ml[2 * pr + 1];
     }
@@ -860,7 +967,7 @@ __global__ __launch_bounds__(256) void rows_weights_kernel(const RowsParams P, i
     }
   }
   __syncthreads();
-  const float* raw = P.raw + (int64_t(b) * P.heads + kvh * P.group) * P.s_c;
+  const float* raw = P.raw + (int64_t(b) * P.heads + kvh * P.group) * P.raw_row;
   const float* in = P.w_in + b * P.wi_sb + kvh * P.wi_sh;
   float* out = P.w_out + b * P.wo_sb + kvh * P.wo_sh;
 #pragma unroll
@@ -870,7 +977,7 @@ __global__ __launch_bounds__(256) void rows_weights_kernel(const RowsParams P, i
     float acc = 0.0f;
     for (int g = 0; g < P.group; ++g)
       acc += sR[g] * __builtin_amdgcn_exp2f(
-                         __builtin_fmaf(raw[int64_t(g) * P.s_c + j], P.scale_log2, -sM[g]));
+                         __builtin_fmaf(raw[g * P.raw_row + j], P.scale_log2, -sM[g]));
     out[j] = in[j] + acc;
   }
 }
@@ -944,7 +1051,7 @@ void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D) {
                   : rows <= 64               ? kTile + 1
                                              : kTile + 2;
   p.prefix_rows = form_rows(p.prefix_form);
-  p.own_rows = form_rows(p.own_form);
+  p.own_rows = int(seq_rows < form_rows(p.own_form) ? seq_rows : form_rows(p.own_form));
 }
 
 hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,

@@ -3,7 +3,7 @@
 The bounds count roundings: a score is a sum of D products in fp32, off by at
 most (D + 2) half steps of the sum of magnitudes, so exp of it (and of the row's
 maximum) by twice that relatively; P is held in two 16-bit parts (the square of
-the type's half step); the exponential, the sums over keys and the division add
+the type's half step), in fp16 it may be one (a half step); the exponential, the sums over keys and the division add
 a few fp32 half steps, taken as 2^-18 in all.  A weighted mean moves by at most
 the weights' relative error times the largest |v|, and again for the divisor.
 """

@@ -34,7 +34,7 @@ def check_out(got, ref, q, ks, vs, scale, label):
         if k.shape[2]:
             rel = max(rel, O.weight_error(q.double(), O.repeat_kv(k.double(), group), scale, dt))
     vmax = max([v.double().abs().amax().item() for v in vs if v.numel()], default=0.0)
-    p16 = (torch.finfo(dt).eps / 2) ** 2
+    p16 = (torch.finfo(dt).eps / 2) ** (2 if dt == BF16 else 1)
     tol = 2 * (rel + p16) * vmax + (torch.finfo(got.dtype).eps / 2) * ref.abs()
     err = (got.double().cpu() - ref).abs()
     print(f"[cached] {label}: err {err.max():.2e} tol {tol.min():.2e}", flush=True)
@@ -65,6 +65,7 @@ PREFIX = [
     (7, 16, 1, 128, 300, 100, 1, FP16, None),           # 112 rows
     (2, 8, 1, 96, 65, 130, 20, FP16, [130, 97]),        # 160 rows of a sequence
     (1, 8, 8, 96, 20000, 600, 1, BF16, None),
+    (130, 2, 1, 64, 40, 260, 1, BF16, [(7 * i) % 261 for i in range(130)]),
     (2, 2, 2, 128, 9000, 300, 40, BF16, [300, 150]),
 ]
 
@@ -174,6 +175,8 @@ ACCUMULATE = [
     (1, 4, 4, 80, 65, BF16, None),
     (2, 4, 2, 64, 0, BF16, None),
     (1, 4, 2, 128, 30000, BF16, None),
+    (70, 4, 2, 64, 400, BF16, [(37 * i) % 401 for i in range(70)]),  # more than 64 sequences
+    (5, 2, 1, 96, 9000, FP16, [0, 9000, 0, 1, 0]),                    # one long among empty ones
 ]
 
 
