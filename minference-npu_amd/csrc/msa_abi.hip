@@ -1323,15 +1323,14 @@ int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const
   // could not cover an item's keys
   const int64_t triples = B * Hkv * rp.n_rto, units = triples * cdiv(Sc, 128);
   const int64_t most = rows_max_chunk(k, v) / 128;  // units of an item
-  rp.min_units = int(std::min<int64_t>(2, most));
-  const int64_t n_own = std::min(cdiv(units, rp.min_units), std::max<int64_t>(512, cdiv(units, most)));
-  const int64_t row_splits = std::min(n_own, cdiv(cdiv(Sc, 128), rp.min_units) + 1);
+  const int64_t n_own = std::min(units, std::max<int64_t>(512, cdiv(units, most)));
+  const int64_t row_splits = std::min(n_own, cdiv(Sc, 128));
   if (rp.n_sp + row_splits > kRowsMaxSplit) return MSA_E_SEQ;
   const int64_t np = cdiv(Hkv * rp.n_sp, 8) * 8 * rp.n_rt;
   if (np + n_own >= (int64_t(1) << 31) || units >= (int64_t(1) << 30)) return MSA_E_HEADS;
   rp.n_own = int(n_own);
-  rp.n_prefix_items = int(np);
-  rp.n_items = int(np + rp.n_own);
+  rp.n_own_wg = int(cdiv(n_own, 8) * 8);
+  rp.n_items = int(np + rp.n_own_wg);
   rp.raw_row = cdiv(Sc, 32) * 32;
   rp.own_row0 = Hkv * rp.n_sp * R;
   return MSA_OK;

@@ -240,8 +240,8 @@ struct RowsParams {
   int prefix_form, own_form;  // of the items (rows_forms), and their rows
   int prefix_rows, own_rows;
   int n_rt, n_sp, chunk_p;   // prefix: row tiles, key splits, keys of a split
-  int n_rto, n_own, min_units;  // own caches: row tiles, items, least units of 128 keys of one
-  int n_prefix_items, n_items;  // prefix: (kv head, split) pairs to a multiple of 8
+  int n_rto, n_own;          // own caches: row tiles, items
+  int n_own_wg, n_items;  // workgroups of the own caches (n_own to a multiple of 8), of all
   float scale_log2;          // softmax scale * log2(e)
   float* part;               // partial O, [row][D]: prefix [kv_heads][n_sp][batch * rows],
                              // from own_row0 on [n_own + batch * kv_heads * n_rto][own_rows]

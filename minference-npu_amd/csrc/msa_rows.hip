@@ -708,7 +708,7 @@ __device__ inline OwnPlan own_plan(const RowsParams& P, bool write) {
       P.plan[1 + b0 + threadIdx.x] = p.total + before;
     p.total += chunk;
   }
-  p.per = uniform(max(P.min_units, (p.total + P.n_own - 1) / P.n_own));
+  p.per = uniform(max(1, (p.total + P.n_own - 1) / P.n_own));
   if (write && threadIdx.x == 0) P.plan[0] = p.per;
   return p;
 }
@@ -745,9 +745,9 @@ __device__ inline void run_item(const RowsParams& P, const Item& it, Shared& sh)
     rows_item<T, D, FORM, CAUSAL, SCORES>(P, it, sh);
 }
 
-// Item blockIdx.x: the prefix items first ((kv head, key range), row tile) in
-// form PF (0: none), then the own-cache items ((sequence, kv head), key range,
-// row tile) in form OF.
+// Workgroups: n_own_wg (a multiple of 8) for the own caches, in form OF, which
+// take longer to start; then the prefix items ((kv head, key range), row tile) in
+// form PF (0: none).
 template <typename T, int D, int PF, int OF, bool CAUSAL, bool SCORES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 128 ? 1 : 2)))
 void rows_kernel(const RowsParams P) {
@@ -757,7 +757,8 @@ void rows_kernel(const RowsParams P) {
   it.raw = nullptr;
   it.raw_row = 0;
   int x = blockIdx.x;
-  if (PF > 0 && x < P.n_prefix_items) {
+  if (PF > 0 && x >= P.n_own_wg) {
+    x -= P.n_own_wg;
     // The row tiles of one (kv head, key range) follow each other on one XCD
     // (workgroup i runs on XCD i % 8), so its L2 serves all but the first.
     const int y = x >> 3, rt = y % P.n_rt;
@@ -782,7 +783,7 @@ void rows_kernel(const RowsParams P) {
   // Own caches: the units of 128 keys of all (sequence, kv head, row tile)
   // triples in a row, cut into equal ranges of P.n_own items, so lengths, known
   // on the device only, do not leave some workgroups with more than others.
-  x -= P.n_prefix_items;
+  if (x >= P.n_own) return;
   const OwnPlan plan = own_plan(P, x == 0);
   const int per_seq = P.kv_heads * P.n_rto;
   int u = x * plan.per;
