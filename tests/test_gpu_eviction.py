@@ -124,6 +124,7 @@ EVICT = [
     (2, 1, 70, 7, 30, 5, 5, [70, 31], BF16),            # rows of 14 bytes
     (1, 2, 300, 96, 300, 10, 4, None, BF16),            # nothing to drop
     (1, 2, 40000, 64, 9000, 1, 1, None, BF16),
+    (2, 1, 70000, 64, 20000, 64, 4, [70000, 65537], BF16),  # more than the registers hold
 ]
 
 
