@@ -414,11 +414,13 @@ int msa_attention_weight_sums(const msa_tensor4* q, const msa_tensor4* k, const 
  *         stride[2] = 1
  *   positions [B][H_kv][keep] int32, contiguous; new_lens [B] int32
  * 1 <= keep <= S, sinks >= 0, recent >= 0, sinks + recent <= keep. */
+/* 0 for S <= 8192: workspace may be NULL */
+size_t msa_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t s);
 int msa_cache_evict(const msa_tensor4* k, const msa_tensor4* v, const msa_tensor4* scores,
                     const int32_t* lens, int64_t keep, int64_t recent, int64_t sinks,
                     const msa_tensor4* k_out, const msa_tensor4* v_out,
                     const msa_tensor4* scores_out, int32_t* positions, int32_t* new_lens,
-                    msa_stream_t stream);
+                    void* workspace, size_t workspace_bytes, msa_stream_t stream);
 
 /* Rotary position embedding of one layer's query and key heads, one launch.
  * Replaces the apply_rotary_pos_emb call of the patched forward

@@ -1543,6 +1543,23 @@ int sums_plan(SumsParams& sp, SumsLayout& l, const msa_tensor4* q, const msa_ten
   return MSA_OK;
 }
 
+// Eviction workspace: histograms and state of rows above 8192 scores, which go in
+// stretches of at least 4096 (8192 where there are 64 rows to fill the GPU: each
+// workgroup reads all the row's histograms).
+struct EvictLayout {
+  size_t state, total;
+  int n_stretch, stretch;
+};
+EvictLayout evict_layout(int64_t rows, int64_t s) {
+  EvictLayout l;
+  const int64_t most = rows >= 64 ? kEvictMaxStretch / 2 : kEvictMaxStretch;
+  l.stretch = int(std::max<int64_t>(4096, cdiv(cdiv(s, most), 64) * 64));
+  l.n_stretch = s <= 8192 ? 0 : int(cdiv(s, l.stretch));
+  l.state = size_t(rows) * l.n_stretch * kEvictBins * 4 * 3;
+  l.total = l.n_stretch == 0 ? 0 : l.state + size_t(rows) * (6 + 3 * kEvictMaxStretch) * 4;
+  return l;
+}
+
 // D contiguous, strides not negative.
 bool evict_rows_ok(const msa_tensor4* t) {
   if (t->size[3] > 1 && t->stride[3] != 1) return false;
@@ -1605,11 +1622,17 @@ int msa_attention_weight_sums(const msa_tensor4* q, const msa_tensor4* k, const 
   return e == hipSuccess ? MSA_OK : int(e);
 }
 
+size_t msa_cache_evict_workspace_bytes(int64_t batch, int64_t kv_heads, int64_t s) {
+  if (batch <= 0 || kv_heads <= 0 || s <= 0 || batch > 65535 || kv_heads > 65535 || s > kMaxSeq)
+    return 0;
+  return evict_layout(batch * kv_heads, s).total;
+}
+
 int msa_cache_evict(const msa_tensor4* k, const msa_tensor4* v, const msa_tensor4* scores,
                     const int32_t* lens, int64_t keep, int64_t recent, int64_t sinks,
                     const msa_tensor4* k_out, const msa_tensor4* v_out,
                     const msa_tensor4* scores_out, int32_t* positions, int32_t* new_lens,
-                    msa_stream_t stream) {
+                    void* workspace, size_t workspace_bytes, msa_stream_t stream) {
   if (!k || !v || !scores || !k_out || !v_out || !scores_out || !positions || !new_lens)
     return MSA_E_NULL;
   const msa_tensor4* ts[4] = {k, v, k_out, v_out};
@@ -1654,6 +1677,13 @@ int msa_cache_evict(const msa_tensor4* k, const msa_tensor4* v, const msa_tensor
   ep.keep = int(keep);
   ep.recent = int(recent);
   ep.sinks = int(sinks);
+  const EvictLayout l = evict_layout(k->size[0] * k->size[1], k->size[2]);
+  if (l.total > 0 && (!workspace || workspace_bytes < l.total)) return MSA_E_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return MSA_E_ALIGN;
+  ep.hist = ws_at<uint32_t>(workspace, 0);
+  ep.state = ws_at<uint32_t>(workspace, l.state);
+  ep.n_stretch = l.n_stretch;
+  ep.stretch = l.stretch;
   ep.unit = 16;
   for (const msa_tensor4* t : ts)
     if (!evict_units16(t)) ep.unit = 2;

@@ -291,7 +291,14 @@ struct EvictParams {
   int64_t s_sb, s_sh, so_sb, so_sh;
   int batch, kv_heads, s, keep, recent, sinks;
   int unit, upr;  // bytes of a copied unit (16 or 2), units of a row
+  // long rows (n_stretch > 0), in stretches of `stretch` keys (a multiple of 64):
+  uint32_t* hist;   // [3 digits][batch * kv_heads][n_stretch][kEvictBins]
+  uint32_t* state;  // [batch * kv_heads][6 + 3 * kEvictMaxStretch]
+  int n_stretch, stretch;
 };
+
+constexpr int kEvictBins = 2048;     // of a digit
+constexpr int kEvictMaxStretch = 16;
 
 // Rotary embedding of one layer's q and k heads (rope_kernel).  q/k/qo/ko
 // strides are [B][H][S][D] element strides; cos/sin are [B or 1][S][rot]

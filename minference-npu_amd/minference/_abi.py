@@ -93,6 +93,7 @@ EXPORTED_SYMBOLS = (
     "msa_decode_accumulate",
     "msa_attention_weight_sums_workspace_bytes",
     "msa_attention_weight_sums",
+    "msa_cache_evict_workspace_bytes",
     "msa_cache_evict",
 )
 
@@ -307,8 +308,10 @@ def load_library() -> ctypes.CDLL:
         lib.msa_cache_evict.restype = ctypes.c_int
         lib.msa_cache_evict.argtypes = [T4] * 3 + [
             ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, T4, T4, T4,
-            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
         ]
+        lib.msa_cache_evict_workspace_bytes.restype = ctypes.c_size_t
+        lib.msa_cache_evict_workspace_bytes.argtypes = [ctypes.c_int64] * 3
         ver = lib.msa_abi_version()
         if ver != ABI_VERSION:
             raise ImportError(f"libmsa ABI version {ver} != expected {ABI_VERSION}")
@@ -397,8 +400,8 @@ def decode_attention_noalloc(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 def _lens_ptr(lens: Optional[torch.Tensor], batch: int, device: torch.device) -> Optional[int]:
     if lens is None:
         return None
-    if (lens.dtype != torch.int32 or tuple(lens.shape) != (batch,) or not lens.is_contiguous()
-            or lens.device != device):
+    if (lens.dtype is not torch.int32 or lens.dim() != 1 or lens.shape[0] != batch
+            or lens.device != device or not lens.is_contiguous()):
         raise ValueError(f"lens must be a contiguous int32 [{batch}] tensor on the caches' device, got "
                          f"{tuple(lens.shape)} {lens.dtype} on {lens.device}")
     return lens.data_ptr()
@@ -413,32 +416,32 @@ def _descriptors(tensors: Sequence[torch.Tensor]) -> list:
     """Addresses of descriptors of [B,H,S,D] tensors, or of [B,H,S] ones as
     [B,H,S,1], in one pack into a buffer of this thread that the next call
     overwrites (six tensors: 4 us, 11 as tensor4 each)."""
-    buf = getattr(_DESCS, "buf", None)
-    if buf is None:
+    try:
+        buf, at = _DESCS.buf, _DESCS.at
+    except AttributeError:  # this thread's first call
         buf = _DESCS.buf = ctypes.create_string_buffer(_TENSOR4.size * _MAX_DESCS)
-        _DESCS.at = [ctypes.addressof(buf) + _TENSOR4.size * i for i in range(_MAX_DESCS)]
+        at = _DESCS.at = [ctypes.addressof(buf) + _TENSOR4.size * i for i in range(_MAX_DESCS)]
     vals = []
     for t in tensors:
-        code = _DTYPE_CODE.get(t.dtype)
-        if code is None:
-            raise TypeError(f"unsupported dtype {t.dtype}")
-        if t.dim() == 4:
-            vals += (t.data_ptr(), *t.shape, *t.stride(), code, 0)
-        elif t.dim() == 3:
-            vals += (t.data_ptr(), *t.shape, 1, *t.stride(), 1, code, 0)
+        sh = t.shape
+        if len(sh) == 4:
+            vals += (t.data_ptr(), *sh, *t.stride(), _DTYPE_CODE[t.dtype], 0)
         else:
-            raise ValueError(f"expected a [B,H,S,D] or [B,H,S] tensor, got {t.dim()}-D")
+            b, h, s = sh
+            sb, sh, ss = t.stride()
+            vals += (t.data_ptr(), b, h, s, 1, sb, sh, ss, 1, _DTYPE_CODE[t.dtype], 0)
     _DESC_PACK[len(tensors)].pack_into(buf, 0, *vals)
-    return _DESCS.at
+    return at
 
 
 def _on_device(device: torch.device, fn) -> None:
     """fn(stream handle) with ``device`` current, on its current stream."""
-    if torch.cuda.current_device() == device.index:
-        fn(current_stream_handle(device))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        fn(torch._C._cuda_getCurrentRawStream(index))  # 0.1 us; current_stream() 2 us
         return
     with torch.cuda.device(device):
-        fn(current_stream_handle(device))
+        fn(torch._C._cuda_getCurrentRawStream(index))
 
 
 def shared_prefix_attention(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, k: torch.Tensor,
@@ -499,9 +502,15 @@ def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
     lib = load_library()
     lens_p = _lens_ptr(lens, k.shape[0], k.device)
     d = _descriptors((k, v, scores, k_out, v_out, scores_out))
-    _on_device(k.device, lambda stream: check(lib.msa_cache_evict(
-        d[0], d[1], d[2], lens_p, keep, recent, sinks, d[3], d[4], d[5], positions.data_ptr(),
-        new_lens.data_ptr(), stream)))
+
+    def launch(stream):
+        need = lib.msa_cache_evict_workspace_bytes(*k.shape[:3])
+        ws = workspace(need, k.device) if need else None
+        check(lib.msa_cache_evict(
+            d[0], d[1], d[2], lens_p, keep, recent, sinks, d[3], d[4], d[5], positions.data_ptr(),
+            new_lens.data_ptr(), ws.data_ptr() if need else None, need, stream))
+
+    _on_device(k.device, launch)
 
 
 def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

@@ -98,8 +98,10 @@ def shared_prefix_attention(
     """
     _check_caches(q, [("prefix", k_prefix, v_prefix, 1), ("own cache", k_cache, v_cache, q.shape[0])])
     s = dense_scale(q.shape[-1]) if scale is None else float(scale)
-    result = make_out(q, out)
-    if out is not None:
+    if out is None:
+        result = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        result = make_out(q, out)
         check_written("out", out)
     if q.numel() == 0:
         return result
@@ -140,16 +142,19 @@ def decode_accumulate(
     _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
     if q.shape[2] != 1:
         raise NotImplementedError("decode_accumulate takes one query row")
-    check_scores("scores", scores, k_cache.shape[:3], k_cache.device)
+    check_scores("scores", scores, k_cache, k_cache.shape[2])
     if scores_out is None:
         scores_out = scores
     else:
-        check_scores("scores_out", scores_out, k_cache.shape[:3], k_cache.device)
-    same = scores_out.data_ptr() == scores.data_ptr() and scores_out.stride() == scores.stride()
+        check_scores("scores_out", scores_out, k_cache, k_cache.shape[2])
+    same = scores_out is scores or (scores_out.data_ptr() == scores.data_ptr()
+                                    and scores_out.stride() == scores.stride())
     check_written("scores_out", scores_out, () if same else (("scores", scores),))
     s = dense_scale(q.shape[-1]) if scale is None else float(scale)
-    result = make_out(q, out)
-    if out is not None:
+    if out is None:
+        result = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        result = make_out(q, out)
         check_written("out", out)
     if q.numel() == 0:
         return result, scores_out

@@ -266,6 +266,8 @@ def _share(t: torch.Tensor, u: torch.Tensor) -> bool:
     and v side by side in one buffer) are told apart exactly; of others, whose
     extents overlap, sharing is assumed."""
     def end(x):
+        if x.is_contiguous():
+            return x.data_ptr() + x.nbytes
         return x.data_ptr() + x.element_size() * (
             1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
 
@@ -295,15 +297,20 @@ def check_written(name: str, t: torch.Tensor, others=()) -> None:
     (name, tensor) ``others``."""
     if t.numel() == 0:
         return
+    if not t.is_contiguous():
+        _check_apart(name, t)
+    for other, u in others:
+        if u.numel() and _share(t, u):
+            raise ValueError(f"{name} shares memory with {other}")
+
+
+def _check_apart(name: str, t: torch.Tensor) -> None:
     span = 0
     for st, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if st <= span:
             raise ValueError(f"{name} has elements that share memory (shape {tuple(t.shape)}, "
                              f"strides {t.stride()})")
         span += st * (n - 1)
-    for other, u in others:
-        if u.numel() and _share(t, u):
-            raise ValueError(f"{name} shares memory with {other}")
 
 
 def head_chunks(n_heads: int):

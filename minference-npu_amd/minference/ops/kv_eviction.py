@@ -22,13 +22,16 @@ __all__ = ["attention_weight_sums", "evict_kv_cache", "check_scores"]
 CACHE_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def check_scores(name: str, t: torch.Tensor, shape, device: torch.device) -> None:
-    """Scores of keys: float32 of ``shape`` [B, H_kv, S], contiguous over S."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != torch.float32:
-        raise ValueError(f"{name} must be float32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
-    if t.device != device:
+def check_scores(name: str, t: torch.Tensor, k: torch.Tensor, n: int) -> None:
+    """Scores of n keys a kv head of the cache k: float32 [B, H_kv, n],
+    contiguous over the keys."""
+    sh, ks = t.shape, k.shape
+    if (len(sh) != 3 or sh[0] != ks[0] or sh[1] != ks[1] or sh[2] != n
+            or t.dtype is not torch.float32):
+        raise ValueError(f"{name} must be float32 {(*ks[:2], n)}, got {t.dtype} {tuple(sh)}")
+    if t.device != k.device:
         raise ValueError(f"{name} must be on the cache's device")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    if n > 1 and t.stride(2) != 1:
         raise ValueError(f"{name} must be contiguous over the keys")
 
 
@@ -63,7 +66,7 @@ def attention_weight_sums(
     check_supported(q, k)
     add = scores is not None
     if add:
-        check_scores("scores", scores, k.shape[:3], k.device)
+        check_scores("scores", scores, k, k.shape[2])
         check_written("scores", scores, (("q", q), ("k", k)))
     else:
         scores = torch.empty(k.shape[:3], dtype=torch.float32, device=k.device)
@@ -122,7 +125,7 @@ def evict_kv_cache(
         raise NotImplementedError(f"caches must both be one of {CACHE_DTYPES}, got "
                                   f"{k_cache.dtype} and {v_cache.dtype}")
     dev = k_cache.device
-    check_scores("scores", scores, (B, H, S), dev)
+    check_scores("scores", scores, k_cache, S)
     if out is None:
         ko, vo = (torch.empty((B, H, keep, D), dtype=k_cache.dtype, device=dev) for _ in range(2))
         so = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
@@ -134,7 +137,7 @@ def evict_kv_cache(
                                  f"got {t.dtype} {tuple(t.shape)} on {t.device}")
             if D > 1 and t.stride(3) != 1:
                 raise ValueError(f"out's {name} must be contiguous over D")
-        check_scores("out's scores", so, (B, H, keep), dev)
+        check_scores("out's scores", so, k_cache, keep)
         ins = [("k_cache", k_cache), ("v_cache", v_cache), ("scores", scores)]
         check_written("out's k", ko, ins)
         check_written("out's v", vo, ins + [("out's k", ko)])

@@ -192,12 +192,14 @@ def test_sums_abi_refusals(kw, want):
     (dict(so=t4([2, 2, 11, 1], F32)), _abi.MSA_E_RANK),
     (dict(k=t4(KV, strides=[9600, 4800, 96, 2])), _abi.MSA_E_ALIGN),
     (dict(pos=None), _abi.MSA_E_NULL),
+    (dict(k=t4([2, 2, 9000, 96]), v=t4([2, 2, 9000, 96]), s=t4([2, 2, 9000, 1], F32), wsb=16),
+     _abi.MSA_E_WORKSPACE),
 ])
 def test_evict_abi_refusals(kw, want):
     lib = _abi.load_library()
     a = dict(k=t4(KV), v=t4(KV), s=t4([2, 2, 50, 1], F32), keep=10, recent=2, sinks=2, ko=t4([2, 2, 10, 96]),
-             vo=t4([2, 2, 10, 96]), so=t4([2, 2, 10, 1], F32), pos=FAKE)
+             vo=t4([2, 2, 10, 96]), so=t4([2, 2, 10, 1], F32), pos=FAKE, wsb=1 << 30)
     a.update(kw)
     st = lib.msa_cache_evict(REF(a["k"]), REF(a["v"]), REF(a["s"]), None, a["keep"], a["recent"], a["sinks"],
-                             REF(a["ko"]), REF(a["vo"]), REF(a["so"]), a["pos"], FAKE, None)
+                             REF(a["ko"]), REF(a["vo"]), REF(a["so"]), a["pos"], FAKE, FAKE, a["wsb"], None)
     assert st == want

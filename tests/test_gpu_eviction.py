@@ -124,7 +124,10 @@ EVICT = [
     (2, 1, 70, 7, 30, 5, 5, [70, 31], BF16),            # rows of 14 bytes
     (1, 2, 300, 96, 300, 10, 4, None, BF16),            # nothing to drop
     (1, 2, 40000, 64, 9000, 1, 1, None, BF16),
-    (2, 1, 70000, 64, 20000, 64, 4, [70000, 65537], BF16),  # more than the registers hold
+    (2, 1, 70000, 64, 20000, 64, 4, [70000, 65537], BF16),
+    (3, 1, 20000, 64, 5000, 4000, 1000, [20000, 5001, 4999], BF16),  # nothing by score
+    (2, 33, 9001, 64, 4500, 100, 4, [9001, 8300], BF16),             # 66 rows, short stretches
+    (1, 1, 300000, 64, 1000, 0, 0, None, BF16),
 ]
 
 
