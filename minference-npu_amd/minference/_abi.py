@@ -425,7 +425,9 @@ def _descriptors(tensors: Sequence[torch.Tensor]) -> list:
     for t in tensors:
         sh = t.shape
         if len(sh) == 4:
-            vals += (t.data_ptr(), *sh, *t.stride(), _DTYPE_CODE[t.dtype], 0)
+            vals += (t.data_ptr(), *sh, *t.stride(), _DTYPE_CODE.get(t.dtype, 0), 0)
+        elif len(sh) != 3:  # a size the library refuses
+            vals += (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
         else:
             b, h, s = sh
             sb, sh, ss = t.stride()
@@ -434,49 +436,53 @@ def _descriptors(tensors: Sequence[torch.Tensor]) -> list:
     return at
 
 
-def _on_device(device: torch.device, fn) -> None:
-    """fn(stream handle) with ``device`` current, on its current stream."""
-    index = device.index
-    if torch._C._cuda_getDevice() == index:
-        fn(torch._C._cuda_getCurrentRawStream(index))  # 0.1 us; current_stream() 2 us
-        return
-    with torch.cuda.device(device):
-        fn(torch._C._cuda_getCurrentRawStream(index))
+class _OnDevice:
+    """The current stream's handle of a device, which is current inside."""
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)  # 0.1 us; current_stream() 2 us
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
 
 
-def shared_prefix_attention(q: torch.Tensor, kp: torch.Tensor, vp: torch.Tensor, k: torch.Tensor,
-                            v: torch.Tensor, out: torch.Tensor, lens: Optional[torch.Tensor],
-                            scale: float) -> None:
-    """Launch msa_shared_prefix_attention on the current stream of q's device:
-    q [B,H,S_q,D] against the prefix kp/vp [1,H_kv,S_p,D] and the own caches
-    k/v [B,H_kv,S_c,D]."""
+def shared_prefix_attention(ts: Sequence[torch.Tensor], out: torch.Tensor,
+                            lens: Optional[torch.Tensor], scale: float) -> int:
+    """msa_shared_prefix_attention on the current stream of q's device, its
+    status: ts = q [B,H,S_q,D], the prefix k and v [1,H_kv,S_p,D], the own caches
+    k and v [B,H_kv,S_c,D], all on one GPU."""
     lib = load_library()
+    q = ts[0]
     lens_p = _lens_ptr(lens, q.shape[0], q.device)
-    d = _descriptors((q, kp, vp, k, v, out))
-
-    def launch(stream):
-        ws = workspace(lib.msa_shared_prefix_workspace_bytes(d[0], d[1], d[2], d[3], d[4]), q.device)
-        check(lib.msa_shared_prefix_attention(d[0], d[1], d[2], d[3], d[4], d[5], lens_p, scale,
-                                              ws.data_ptr(), ws.numel(), stream))
-
-    _on_device(q.device, launch)
+    d = _descriptors((*ts, out))
+    with _OnDevice(q.get_device()) as stream:
+        n = lib.msa_shared_prefix_workspace_bytes(d[0], d[1], d[2], d[3], d[4])
+        ws = torch.empty(n or 256, dtype=torch.uint8, device=q.device)
+        return lib.msa_shared_prefix_attention(d[0], d[1], d[2], d[3], d[4], d[5], lens_p, scale,
+                                               ws.data_ptr(), n, stream)
 
 
-def decode_accumulate(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
-                      lens: Optional[torch.Tensor], scores: torch.Tensor,
-                      scores_out: torch.Tensor, scale: float) -> None:
-    """Launch msa_decode_accumulate on the current stream of q's device: q
-    [B,H,1,D] against the cache k/v; scores and scores_out fp32 [B,H_kv,S]."""
+def decode_accumulate(ts: Sequence[torch.Tensor], out: torch.Tensor, lens: Optional[torch.Tensor],
+                      scores: torch.Tensor, scores_out: torch.Tensor, scale: float) -> int:
+    """msa_decode_accumulate on the current stream of q's device, its status: ts
+    = q [B,H,1,D] and the cache's k and v, all on one GPU; scores and scores_out
+    fp32 [B,H_kv,S]."""
     lib = load_library()
+    q = ts[0]
     lens_p = _lens_ptr(lens, q.shape[0], q.device)
-    d = _descriptors((q, k, v, out, scores, scores_out))
-
-    def launch(stream):
-        ws = workspace(lib.msa_decode_accumulate_workspace_bytes(d[0], d[1], d[2]), q.device)
-        check(lib.msa_decode_accumulate(d[0], d[1], d[2], d[3], lens_p, d[4], d[5], scale,
-                                        ws.data_ptr(), ws.numel(), stream))
-
-    _on_device(q.device, launch)
+    d = _descriptors((*ts, out, scores, scores_out))
+    with _OnDevice(q.get_device()) as stream:
+        n = lib.msa_decode_accumulate_workspace_bytes(d[0], d[1], d[2])
+        ws = torch.empty(n or 256, dtype=torch.uint8, device=q.device)
+        return lib.msa_decode_accumulate(d[0], d[1], d[2], d[3], lens_p, d[4], d[5], scale,
+                                         ws.data_ptr(), n, stream)
 
 
 def attention_weight_sums(q: torch.Tensor, k: torch.Tensor, sums: torch.Tensor, add: bool,
@@ -485,13 +491,11 @@ def attention_weight_sums(q: torch.Tensor, k: torch.Tensor, sums: torch.Tensor, 
     sums fp32 [B,H_kv,S_k], added to when ``add``."""
     lib = load_library()
     d = _descriptors((q, k, sums))
-
-    def launch(stream):
-        ws = workspace(lib.msa_attention_weight_sums_workspace_bytes(d[0], d[1]), q.device)
-        check(lib.msa_attention_weight_sums(d[0], d[1], d[2], int(add), scale, ws.data_ptr(),
-                                            ws.numel(), stream))
-
-    _on_device(q.device, launch)
+    with _OnDevice(q.get_device()) as stream:
+        n = lib.msa_attention_weight_sums_workspace_bytes(d[0], d[1])
+        ws = torch.empty(n or 256, dtype=torch.uint8, device=q.device)
+        check(lib.msa_attention_weight_sums(d[0], d[1], d[2], int(add), scale, ws.data_ptr(), n,
+                                            stream))
 
 
 def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
@@ -502,15 +506,12 @@ def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
     lib = load_library()
     lens_p = _lens_ptr(lens, k.shape[0], k.device)
     d = _descriptors((k, v, scores, k_out, v_out, scores_out))
-
-    def launch(stream):
-        need = lib.msa_cache_evict_workspace_bytes(*k.shape[:3])
-        ws = workspace(need, k.device) if need else None
+    with _OnDevice(k.get_device()) as stream:
+        n = lib.msa_cache_evict_workspace_bytes(*k.shape[:3])
+        ws = torch.empty(n, dtype=torch.uint8, device=k.device) if n else None
         check(lib.msa_cache_evict(
             d[0], d[1], d[2], lens_p, keep, recent, sinks, d[3], d[4], d[5], positions.data_ptr(),
-            new_lens.data_ptr(), ws.data_ptr() if need else None, need, stream))
-
-    _on_device(k.device, launch)
+            new_lens.data_ptr(), ws.data_ptr() if n else None, n, stream))
 
 
 def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

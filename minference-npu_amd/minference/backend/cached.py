@@ -51,17 +51,38 @@ def _check_caches(q: torch.Tensor, pairs) -> None:
         raise ValueError("head_dim must be positive")
 
 
-def _padded(ts, out: torch.Tensor, fn) -> None:
-    """fn(views of ts, out) at the kernel head dim of ts[0]; other head dims
-    are zero-padded to it (no dot product changes) and cut again."""
+def _launch(fn, ts, out: torch.Tensor, explain) -> None:
+    """fn(ts, out) -> status, on the tensors as they are where the library takes
+    them.  Otherwise ``explain`` raises the error of arguments that fit nowhere;
+    what is left are rows that are not aligned (copied) and head dims the kernels
+    are not built for (zero-padded, which changes no dot product, and cut
+    again)."""
+    device = ts[0].get_device()
+    if device >= 0 and all(t.get_device() == device for t in ts):
+        status = fn(ts, out)
+        if status == _abi.MSA_OK:
+            return
+    else:
+        status = _abi.MSA_E_NULL
+    explain()
+    if status == _abi.MSA_E_ALIGN:
+        _abi.check(fn([kernel_view(t) for t in ts], out))
+        return
     d = ts[0].shape[3]
     dk = kernel_head_dim(d)
     if dk == d:
-        fn([kernel_view(t) for t in ts], out)
-        return
+        _abi.check(status)
     tmp = torch.empty((*out.shape[:3], dk), dtype=out.dtype, device=out.device)
-    fn([pad_head_dim(t, dk) for t in ts], tmp)
+    _abi.check(fn([pad_head_dim(t, dk) for t in ts], tmp))
     out.copy_(tmp[..., :d])
+
+
+def _output(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    make_out(q, out)
+    check_written("out", out)
+    return out
 
 
 @accepts_float32(("q", "k_prefix", "v_prefix", "k_cache", "v_cache"))
@@ -96,17 +117,17 @@ def shared_prefix_attention(
     S_q), not once per sequence.  Equal to dense attention over the
     concatenated caches.  A row that sees no key, or only scores of -inf, is 0.
     """
-    _check_caches(q, [("prefix", k_prefix, v_prefix, 1), ("own cache", k_cache, v_cache, q.shape[0])])
-    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
-    if out is None:
-        result = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        result = make_out(q, out)
-        check_written("out", out)
-    if q.numel() == 0:
-        return result
-    _padded((q, k_prefix, v_prefix, k_cache, v_cache), result,
-            lambda ts, r: _abi.shared_prefix_attention(*ts, r, lens, s))
+    def explain():
+        _check_caches(q, [("prefix", k_prefix, v_prefix, 1),
+                          ("own cache", k_cache, v_cache, q.shape[0])])
+
+    if q.dim() != 4 or q.numel() == 0:
+        explain()
+        return _output(q, out)
+    s = dense_scale(q.shape[3]) if scale is None else float(scale)
+    result = _output(q, out)
+    _launch(lambda ts, r: _abi.shared_prefix_attention(ts, r, lens, s),
+            (q, k_prefix, v_prefix, k_cache, v_cache), result, explain)
     return result
 
 
@@ -139,25 +160,25 @@ def decode_accumulate(
     Returns (out, scores_out).  The same call gives the same bits.  With lens[b]
     = 0, or only scores of -inf, a row is 0 and adds nothing.
     """
-    _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
-    if q.shape[2] != 1:
-        raise NotImplementedError("decode_accumulate takes one query row")
+    def explain():
+        _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
+        if q.shape[2] != 1:
+            raise NotImplementedError("decode_accumulate takes one query row")
+
+    if q.dim() != 4 or k_cache.dim() != 4 or q.numel() == 0 or not q.is_cuda:
+        explain()
     check_scores("scores", scores, k_cache, k_cache.shape[2])
     if scores_out is None:
         scores_out = scores
-    else:
+    elif scores_out is not scores:
         check_scores("scores_out", scores_out, k_cache, k_cache.shape[2])
     same = scores_out is scores or (scores_out.data_ptr() == scores.data_ptr()
                                     and scores_out.stride() == scores.stride())
     check_written("scores_out", scores_out, () if same else (("scores", scores),))
-    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
-    if out is None:
-        result = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    else:
-        result = make_out(q, out)
-        check_written("out", out)
+    result = _output(q, out)
     if q.numel() == 0:
         return result, scores_out
-    _padded((q, k_cache, v_cache), result,
-            lambda ts, r: _abi.decode_accumulate(*ts, r, lens, scores, scores_out, s))
+    s = dense_scale(q.shape[3]) if scale is None else float(scale)
+    _launch(lambda ts, r: _abi.decode_accumulate(ts, r, lens, scores, scores_out, s),
+            (q, k_cache, v_cache), result, explain)
     return result, scores_out
