@@ -355,11 +355,6 @@ void sums_cols_kernel(const SumsParams P) {
   const float c = P.scale_log2;
   const bool active = j0 < P.s_k;
 
-  u32x4 kb[NT][NKS];
-  hold_rows<D, NT>(reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + int64_t(kvh) * P.k_sh +
-                       int64_t(min(j0, P.s_k - 1)) * P.k_ss,
-                   P.s_k - j0, P.k_ss, lane, lds + w * Part::BYTES, kb);
-
   // 64-row tiles from the first row that sees the item's first key (to 16), of
   // every head of the kv head
   const int rb = max(0, 4 * kt * TK - shift) / 16 * 16;
@@ -393,6 +388,12 @@ void sums_cols_kernel(const SumsParams P) {
     part.store(lds + stage * Shape::STAGE + w * Part::BYTES, qr);
     if (lane < 32) stat[slot][lane >> 4][16 * w + lc] = st;
   };
+
+  if (t1 > t0) load();  // in flight under the held keys
+  u32x4 kb[NT][NKS];
+  hold_rows<D, NT>(reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + int64_t(kvh) * P.k_sh +
+                       int64_t(min(j0, P.s_k - 1)) * P.k_ss,
+                   P.s_k - j0, P.k_ss, lane, lds + w * Part::BYTES, kb);
 
   float acc[NT], sum[NT];
 #pragma unroll
@@ -436,7 +437,6 @@ void sums_cols_kernel(const SumsParams P) {
   };
 
   if (t1 > t0) {
-    load();
     __syncthreads();  // the held keys have left LDS
     store(0, 0);
     load();
