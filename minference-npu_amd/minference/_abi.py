@@ -10,6 +10,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
 import os
 import struct
 import threading
@@ -17,7 +19,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from ._build import LIB_PATH
+from ._build import CALLS_PATH, LIB_PATH
 
 # status codes (include/msa.h)
 MSA_OK = 0
@@ -397,121 +399,45 @@ def decode_attention_noalloc(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         current_stream_handle(q.device)))
 
 
-def _lens_ptr(lens: Optional[torch.Tensor], batch: int, device: torch.device) -> Optional[int]:
-    if lens is None:
-        return None
-    if (lens.dtype is not torch.int32 or lens.dim() != 1 or lens.shape[0] != batch
-            or lens.device != device or not lens.is_contiguous()):
+_CALLS = None
+
+
+def calls():
+    """The _msa_calls module (csrc/msa_calls.cpp), bound to the loaded library:
+    the cache operators' calls.  Its functions return their outputs, a status of
+    the library, or None for arguments it has no descriptor for."""
+    global _CALLS
+    if _CALLS is None:
+        lib = load_library()
+        if not os.path.exists(CALLS_PATH):
+            raise ImportError(f"{CALLS_PATH} not found; build it with `python -m minference._build` "
+                              "(run from minference-npu_amd/)")
+        loader = importlib.machinery.ExtensionFileLoader("_msa_calls", CALLS_PATH)
+        spec = importlib.util.spec_from_file_location("_msa_calls", CALLS_PATH, loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, "msa_" + n), ctypes.c_void_p).value for n in (
+            "shared_prefix_workspace_bytes", "shared_prefix_attention",
+            "decode_accumulate_workspace_bytes", "decode_accumulate",
+            "attention_weight_sums_workspace_bytes", "attention_weight_sums",
+            "cache_evict_workspace_bytes", "cache_evict")))
+        _CALLS = module
+    return _CALLS
+
+
+def check_call(result) -> None:
+    """Raises for a result of calls() that is no output."""
+    if result is None:
+        raise ValueError("the library takes strided GPU tensors of one device")
+    if result.__class__ is int:
+        check(result)
+
+
+def check_lens(lens: Optional[torch.Tensor], batch: int, device: torch.device) -> None:
+    if lens is not None and (lens.dtype != torch.int32 or tuple(lens.shape) != (batch,)
+                             or not lens.is_contiguous() or lens.device != device):
         raise ValueError(f"lens must be a contiguous int32 [{batch}] tensor on the caches' device, got "
                          f"{tuple(lens.shape)} {lens.dtype} on {lens.device}")
-    return lens.data_ptr()
-
-
-_MAX_DESCS = 8
-_DESC_PACK = [struct.Struct("@" + "P4q4qii" * n) for n in range(_MAX_DESCS + 1)]
-_DESCS = threading.local()
-
-
-def _descriptors(tensors: Sequence[torch.Tensor]) -> list:
-    """Addresses of descriptors of [B,H,S,D] tensors, or of [B,H,S] ones as
-    [B,H,S,1], in one pack into a buffer of this thread that the next call
-    overwrites (six tensors: 4 us, 11 as tensor4 each)."""
-    try:
-        buf, at = _DESCS.buf, _DESCS.at
-    except AttributeError:  # this thread's first call
-        buf = _DESCS.buf = ctypes.create_string_buffer(_TENSOR4.size * _MAX_DESCS)
-        at = _DESCS.at = [ctypes.addressof(buf) + _TENSOR4.size * i for i in range(_MAX_DESCS)]
-    vals = []
-    for t in tensors:
-        sh = t.shape
-        if len(sh) == 4:
-            vals += (t.data_ptr(), *sh, *t.stride(), _DTYPE_CODE.get(t.dtype, 0), 0)
-        elif len(sh) != 3:  # a size the library refuses
-            vals += (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-        else:
-            b, h, s = sh
-            sb, sh, ss = t.stride()
-            vals += (t.data_ptr(), b, h, s, 1, sb, sh, ss, 1, _DTYPE_CODE[t.dtype], 0)
-    _DESC_PACK[len(tensors)].pack_into(buf, 0, *vals)
-    return at
-
-
-class _OnDevice:
-    """The current stream's handle of a device, which is current inside."""
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self) -> int:
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)  # 0.1 us; current_stream() 2 us
-
-    def __exit__(self, *exc) -> None:
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-
-
-def shared_prefix_attention(ts: Sequence[torch.Tensor], out: torch.Tensor,
-                            lens: Optional[torch.Tensor], scale: float) -> int:
-    """msa_shared_prefix_attention on the current stream of q's device, its
-    status: ts = q [B,H,S_q,D], the prefix k and v [1,H_kv,S_p,D], the own caches
-    k and v [B,H_kv,S_c,D], all on one GPU."""
-    lib = load_library()
-    q = ts[0]
-    lens_p = _lens_ptr(lens, q.shape[0], q.device)
-    d = _descriptors((*ts, out))
-    with _OnDevice(q.get_device()) as stream:
-        n = lib.msa_shared_prefix_workspace_bytes(d[0], d[1], d[2], d[3], d[4])
-        ws = torch.empty(n or 256, dtype=torch.uint8, device=q.device)
-        return lib.msa_shared_prefix_attention(d[0], d[1], d[2], d[3], d[4], d[5], lens_p, scale,
-                                               ws.data_ptr(), n, stream)
-
-
-def decode_accumulate(ts: Sequence[torch.Tensor], out: torch.Tensor, lens: Optional[torch.Tensor],
-                      scores: torch.Tensor, scores_out: torch.Tensor, scale: float) -> int:
-    """msa_decode_accumulate on the current stream of q's device, its status: ts
-    = q [B,H,1,D] and the cache's k and v, all on one GPU; scores and scores_out
-    fp32 [B,H_kv,S]."""
-    lib = load_library()
-    q = ts[0]
-    lens_p = _lens_ptr(lens, q.shape[0], q.device)
-    d = _descriptors((*ts, out, scores, scores_out))
-    with _OnDevice(q.get_device()) as stream:
-        n = lib.msa_decode_accumulate_workspace_bytes(d[0], d[1], d[2])
-        ws = torch.empty(n or 256, dtype=torch.uint8, device=q.device)
-        return lib.msa_decode_accumulate(d[0], d[1], d[2], d[3], lens_p, d[4], d[5], scale,
-                                         ws.data_ptr(), n, stream)
-
-
-def attention_weight_sums(q: torch.Tensor, k: torch.Tensor, sums: torch.Tensor, add: bool,
-                          scale: float) -> None:
-    """Launch msa_attention_weight_sums on the current stream of q's device:
-    sums fp32 [B,H_kv,S_k], added to when ``add``."""
-    lib = load_library()
-    d = _descriptors((q, k, sums))
-    with _OnDevice(q.get_device()) as stream:
-        n = lib.msa_attention_weight_sums_workspace_bytes(d[0], d[1])
-        ws = torch.empty(n or 256, dtype=torch.uint8, device=q.device)
-        check(lib.msa_attention_weight_sums(d[0], d[1], d[2], int(add), scale, ws.data_ptr(), n,
-                                            stream))
-
-
-def cache_evict(k: torch.Tensor, v: torch.Tensor, scores: torch.Tensor,
-                lens: Optional[torch.Tensor], keep: int, recent: int, sinks: int,
-                k_out: torch.Tensor, v_out: torch.Tensor, scores_out: torch.Tensor,
-                positions: torch.Tensor, new_lens: torch.Tensor) -> None:
-    """Launch msa_cache_evict on the current stream of k's device."""
-    lib = load_library()
-    lens_p = _lens_ptr(lens, k.shape[0], k.device)
-    d = _descriptors((k, v, scores, k_out, v_out, scores_out))
-    with _OnDevice(k.get_device()) as stream:
-        n = lib.msa_cache_evict_workspace_bytes(*k.shape[:3])
-        ws = torch.empty(n, dtype=torch.uint8, device=k.device) if n else None
-        check(lib.msa_cache_evict(
-            d[0], d[1], d[2], lens_p, keep, recent, sinks, d[3], d[4], d[5], positions.data_ptr(),
-            new_lens.data_ptr(), ws.data_ptr() if n else None, n, stream))
 
 
 def rope_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,

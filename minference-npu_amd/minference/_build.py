@@ -1,4 +1,5 @@
-"""Build libmsa.so (the HIP kernels + C ABI) in-tree for gfx950.
+"""Build libmsa.so (the HIP kernels + C ABI) in-tree for gfx950, and _msa_calls.so
+(host code: the cache operators' calls from Python).
 
     python -m minference._build          (from minference-npu_amd/)
 
@@ -12,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
@@ -19,6 +21,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC_DIR = os.path.join(os.path.dirname(PKG_DIR), "csrc")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libmsa.so")
+CALLS_PATH = os.path.join(LIB_DIR, "_msa_calls.so")
 
 SOURCES = ("msa_abi.hip", "msa_estimator.hip", "msa_attention.hip", "msa_decode.hip", "msa_vs.hip",
            "msa_rope.hip", "msa_round.hip", "msa_rows.hip",
@@ -52,9 +55,30 @@ def _run(cmd: list) -> subprocess.CompletedProcess:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(
-            "hipcc failed (%d):\n%s\n%s" % (proc.returncode, " ".join(cmd), proc.stderr)
+            "compiler failed (%d):\n%s\n%s" % (proc.returncode, " ".join(cmd), proc.stderr)
         )
     return proc
+
+
+def build_calls(out_path: str = CALLS_PATH) -> str:
+    """Compile the Python module of the cache operators' calls (host code
+    against torch's headers) next to the library; returns its path."""
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    os.makedirs(os.path.dirname(os.path.abspath(out_path)), exist_ok=True)
+    tmp = out_path + ".tmp"
+    _run([shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared",
+          "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          "-I", os.path.join(root, "include"),
+          "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+          "-I", os.path.join(rocm, "include"), "-I", sysconfig.get_paths()["include"],
+          "-o", tmp, os.path.join(CSRC_DIR, "msa_calls.cpp"), "-L", os.path.join(root, "lib"),
+          "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"])
+    os.replace(tmp, out_path)
+    return out_path
 
 
 def build(verbose: bool = False, extra_flags: tuple[str, ...] = (), csrc_dir: str = CSRC_DIR,
@@ -73,7 +97,10 @@ def build(verbose: bool = False, extra_flags: tuple[str, ...] = (), csrc_dir: st
         cmds = [[hipcc, *HIPCC_FLAGS, *extra_flags, "-c", "-o", o, os.path.join(csrc_dir, s)]
                 for s, o in zip(SOURCES, objs)]
         with ThreadPoolExecutor(max_workers=jobs) as pool:
+            calls = pool.submit(build_calls) if out_path == LIB_PATH else None
             procs = list(pool.map(_run, cmds))
+            if calls is not None:
+                calls.result()
         tmp = out_path + ".tmp"
         procs.append(_run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp, *objs]))
     if verbose:

@@ -51,38 +51,29 @@ def _check_caches(q: torch.Tensor, pairs) -> None:
         raise ValueError("head_dim must be positive")
 
 
-def _launch(fn, ts, out: torch.Tensor, explain) -> None:
-    """fn(ts, out) -> status, on the tensors as they are where the library takes
-    them.  Otherwise ``explain`` raises the error of arguments that fit nowhere;
-    what is left are rows that are not aligned (copied) and head dims the kernels
-    are not built for (zero-padded, which changes no dot product, and cut
-    again)."""
-    device = ts[0].get_device()
-    if device >= 0 and all(t.get_device() == device for t in ts):
-        status = fn(ts, out)
-        if status == _abi.MSA_OK:
-            return
-    else:
-        status = _abi.MSA_E_NULL
-    explain()
-    if status == _abi.MSA_E_ALIGN:
-        _abi.check(fn([kernel_view(t) for t in ts], out))
-        return
-    d = ts[0].shape[3]
+def _finish(result, call, ts, q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+    """The output of valid arguments that the library did not take as they are
+    (``result``: its status): rows that are not aligned are copied, head dims the
+    kernels are not built for are zero-padded (no dot product changes) and cut
+    again."""
+    d = q.shape[3]
     dk = kernel_head_dim(d)
-    if dk == d:
-        _abi.check(status)
-    tmp = torch.empty((*out.shape[:3], dk), dtype=out.dtype, device=out.device)
-    _abi.check(fn([pad_head_dim(t, dk) for t in ts], tmp))
-    out.copy_(tmp[..., :d])
+    if result.__class__ is int and result < 0 and dk != d:
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        tmp = call([pad_head_dim(t, dk) for t in ts],
+                   torch.empty((*q.shape[:3], dk), dtype=out.dtype, device=q.device))
+        _abi.check_call(tmp)
+        return out.copy_(tmp[..., :d])
+    if result == _abi.MSA_E_ALIGN:
+        result = call([kernel_view(t) for t in ts], out)
+    _abi.check_call(result)
+    return result
 
 
-def _output(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
-    if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+def _check_out(q: torch.Tensor, out: torch.Tensor) -> None:
     make_out(q, out)
     check_written("out", out)
-    return out
 
 
 @accepts_float32(("q", "k_prefix", "v_prefix", "k_cache", "v_cache"))
@@ -117,18 +108,22 @@ def shared_prefix_attention(
     S_q), not once per sequence.  Equal to dense attention over the
     concatenated caches.  A row that sees no key, or only scores of -inf, is 0.
     """
-    def explain():
-        _check_caches(q, [("prefix", k_prefix, v_prefix, 1),
-                          ("own cache", k_cache, v_cache, q.shape[0])])
+    if out is not None:
+        _check_out(q, out)
+    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
 
-    if q.dim() != 4 or q.numel() == 0:
-        explain()
-        return _output(q, out)
-    s = dense_scale(q.shape[3]) if scale is None else float(scale)
-    result = _output(q, out)
-    _launch(lambda ts, r: _abi.shared_prefix_attention(ts, r, lens, s),
-            (q, k_prefix, v_prefix, k_cache, v_cache), result, explain)
-    return result
+    def call(ts, result):
+        return _abi.calls().shared_prefix(*ts, result, lens, s)
+
+    ts = (q, k_prefix, v_prefix, k_cache, v_cache)
+    result = call(ts, out)
+    if result is not None and result.__class__ is not int:
+        return result
+    _check_caches(q, [("prefix", k_prefix, v_prefix, 1), ("own cache", k_cache, v_cache, q.shape[0])])
+    _abi.check_lens(lens, q.shape[0], q.device)
+    if q.numel() == 0:
+        return torch.empty_like(q) if out is None else out
+    return _finish(result, call, ts, q, out)
 
 
 @accepts_float32(("q", "k_cache", "v_cache"), once=True)
@@ -160,25 +155,32 @@ def decode_accumulate(
     Returns (out, scores_out).  The same call gives the same bits.  With lens[b]
     = 0, or only scores of -inf, a row is 0 and adds nothing.
     """
-    def explain():
+    if k_cache.dim() != 4 or not q.is_cuda:
         _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
-        if q.shape[2] != 1:
-            raise NotImplementedError("decode_accumulate takes one query row")
-
-    if q.dim() != 4 or k_cache.dim() != 4 or q.numel() == 0 or not q.is_cuda:
-        explain()
     check_scores("scores", scores, k_cache, k_cache.shape[2])
-    if scores_out is None:
+    if scores_out is None or scores_out is scores:
         scores_out = scores
-    elif scores_out is not scores:
+        check_written("scores", scores)
+    else:
         check_scores("scores_out", scores_out, k_cache, k_cache.shape[2])
-    same = scores_out is scores or (scores_out.data_ptr() == scores.data_ptr()
-                                    and scores_out.stride() == scores.stride())
-    check_written("scores_out", scores_out, () if same else (("scores", scores),))
-    result = _output(q, out)
-    if q.numel() == 0:
+        same = (scores_out.data_ptr() == scores.data_ptr()
+                and scores_out.stride() == scores.stride())
+        check_written("scores_out", scores_out, () if same else (("scores", scores),))
+    if out is not None:
+        _check_out(q, out)
+    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
+
+    def call(ts, result):
+        return _abi.calls().decode_accumulate(*ts, result, lens, scores, scores_out, s)
+
+    ts = (q, k_cache, v_cache)
+    result = call(ts, out)
+    if result is not None and result.__class__ is not int:
         return result, scores_out
-    s = dense_scale(q.shape[3]) if scale is None else float(scale)
-    _launch(lambda ts, r: _abi.decode_accumulate(ts, r, lens, scores, scores_out, s),
-            (q, k_cache, v_cache), result, explain)
-    return result, scores_out
+    _check_caches(q, [("cache", k_cache, v_cache, q.shape[0])])
+    if q.shape[2] != 1:
+        raise NotImplementedError("decode_accumulate takes one query row")
+    _abi.check_lens(lens, q.shape[0], q.device)
+    if q.numel() == 0:
+        return torch.empty_like(q) if out is None else out, scores_out
+    return _finish(result, call, ts, q, out), scores_out

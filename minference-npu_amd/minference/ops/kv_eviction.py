@@ -58,28 +58,31 @@ def attention_weight_sums(
     key j.  The same call gives the same bits.  Rows with only scores of -inf
     add nothing.
     """
+    if scores is not None:
+        if k.dim() == 4:
+            check_scores("scores", scores, k, k.shape[2])
+        check_written("scores", scores, (("q", q), ("k", k)))
+    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
+    result = _abi.calls().weight_sums(q, k, scores, s)
+    if result is not None and result.__class__ is not int:
+        return result
+    # not taken as they are: why, or copies that are
     if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError(f"q [B,H,S_q,D] and k [B,H_kv,S_k,D] expected, got {tuple(q.shape)} and "
                          f"{tuple(k.shape)}")
     if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
         raise ValueError(f"q heads {q.shape[1]} not a multiple of k heads {k.shape[1]}")
     check_supported(q, k)
-    add = scores is not None
-    if add:
-        check_scores("scores", scores, k, k.shape[2])
-        check_written("scores", scores, (("q", q), ("k", k)))
-    else:
-        scores = torch.empty(k.shape[:3], dtype=torch.float32, device=k.device)
     if q.numel() == 0:
-        return scores if add else scores.zero_()
-    s = dense_scale(q.shape[-1]) if scale is None else float(scale)
+        return scores if scores is not None else torch.zeros(k.shape[:3], dtype=torch.float32,
+                                                             device=k.device)
     dk = kernel_head_dim(q.shape[3])
-    if dk == q.shape[3]:
-        q, k = kernel_view(q), kernel_view(k)
-    else:
-        q, k = pad_head_dim(q, dk), pad_head_dim(k, dk)
-    _abi.attention_weight_sums(q, k, scores, add, s)
-    return scores
+    if result.__class__ is int and result < 0 and dk != q.shape[3]:
+        result = _abi.calls().weight_sums(pad_head_dim(q, dk), pad_head_dim(k, dk), scores, s)
+    elif result == _abi.MSA_E_ALIGN:
+        result = _abi.calls().weight_sums(kernel_view(q), kernel_view(k), scores, s)
+    _abi.check_call(result)
+    return result
 
 
 def evict_kv_cache(
@@ -113,6 +116,13 @@ def evict_kv_cache(
     int32 ``[B, H_kv, keep]`` positions they had, and the int32 ``[B]`` lengths,
     min(lens, keep).  Rows behind a shorter sequence are 0, their positions -1.
     """
+    outs = (None, None, None)
+    if out is not None:
+        outs = _check_outs(k_cache, v_cache, scores, keep, out)
+    result = _abi.calls().evict(k_cache, v_cache, scores, lens, keep, recent, sinks, *outs)
+    if result.__class__ is tuple:
+        return result
+    # not taken as they are: why, or copies that are
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"k_cache and v_cache must be [B,H_kv,S,D] of one shape, got "
                          f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
@@ -124,32 +134,30 @@ def evict_kv_cache(
     if k_cache.dtype not in CACHE_DTYPES or v_cache.dtype != k_cache.dtype:
         raise NotImplementedError(f"caches must both be one of {CACHE_DTYPES}, got "
                                   f"{k_cache.dtype} and {v_cache.dtype}")
-    dev = k_cache.device
     check_scores("scores", scores, k_cache, S)
-    if out is None:
-        ko, vo = (torch.empty((B, H, keep, D), dtype=k_cache.dtype, device=dev) for _ in range(2))
-        so = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
-    else:
-        ko, vo, so = out
-        for name, t in (("k", ko), ("v", vo)):
-            if tuple(t.shape) != (B, H, keep, D) or t.dtype != k_cache.dtype or t.device != dev:
-                raise ValueError(f"out's {name} must be {k_cache.dtype} {(B, H, keep, D)} on {dev}, "
-                                 f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-            if D > 1 and t.stride(3) != 1:
-                raise ValueError(f"out's {name} must be contiguous over D")
-        check_scores("out's scores", so, k_cache, keep)
-        ins = [("k_cache", k_cache), ("v_cache", v_cache), ("scores", scores)]
-        check_written("out's k", ko, ins)
-        check_written("out's v", vo, ins + [("out's k", ko)])
-        check_written("out's scores", so, ins + [("out's k", ko), ("out's v", vo)])
-    pos = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    _abi.check_lens(lens, B, k_cache.device)
     if k_cache.numel() == 0:
         raise ValueError(f"the caches are empty: {tuple(k_cache.shape)}")
-    if D > 1 and k_cache.stride(3) != 1:
-        k_cache = k_cache.contiguous()
-    if D > 1 and v_cache.stride(3) != 1:
-        v_cache = v_cache.contiguous()
-    _abi.cache_evict(k_cache, v_cache, scores, lens, int(keep), int(recent), int(sinks), ko, vo, so,
-                     pos, new_lens)
-    return ko, vo, so, pos, new_lens
+    if result == _abi.MSA_E_ALIGN:
+        result = _abi.calls().evict(k_cache.contiguous(), v_cache.contiguous(), scores, lens, keep,
+                                    recent, sinks, *outs)
+    _abi.check_call(result)
+    return result
+
+
+def _check_outs(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, keep: int, out):
+    """evict_kv_cache's outputs: shapes, types, and apart from all else."""
+    ko, vo, so = out
+    want = (*k_cache.shape[:2], keep, *k_cache.shape[3:])
+    for name, t in (("k", ko), ("v", vo)):
+        if tuple(t.shape) != want or t.dtype != k_cache.dtype or t.device != k_cache.device:
+            raise ValueError(f"out's {name} must be {k_cache.dtype} {want} on {k_cache.device}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"out's {name} must be contiguous over D")
+    check_scores("out's scores", so, k_cache, keep)
+    ins = [("k_cache", k_cache), ("v_cache", v_cache), ("scores", scores)]
+    check_written("out's k", ko, ins)
+    check_written("out's v", vo, ins + [("out's k", ko)])
+    check_written("out's scores", so, ins + [("out's k", ko), ("out's v", vo)])
+    return ko, vo, so
