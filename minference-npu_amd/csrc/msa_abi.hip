@@ -1518,19 +1518,28 @@ int sums_plan(SumsParams& sp, SumsLayout& l, const msa_tensor4* q, const msa_ten
   sp.s_k = int(Sk);
   sp.s_q_pad = int(cdiv(Sq, 16) * 16);
   const int tiles = sums_tiles(int(D));
-  sp.share = Sq > 16 * tiles;
+  // Stats: four waves on 256 rows share the keys they read; where that leaves few
+  // 256 x 256 blocks (4096: 16 a CU), 64 rows an item, its waves on different keys.
+  // us with / without sharing: 16 heads x 225 rows 34 / 28, 16 x 165 of 327 keys
+  // 23 / 16, 16 x 323 of 4244 41 / 33, 32 x 1052 47 / 46, all from 8192 blocks on
+  // faster with.
+  sp.share = Sq > 16 * tiles && BH * cdiv(Sq, 64 * tiles) * cdiv(Sk, 256) >= 4096;
   sp.stat_rows = sp.share ? 64 * tiles : Sq <= 16 ? 16 : 16 * tiles;
   sp.n_rt = int(cdiv(Sq, sp.stat_rows));
-  // stats: key splits where there are few items
+  // key splits up to 768 items (three a CU), of at least 256 keys; each is a
+  // (m, l) a row to merge: 2304 items of 512 keys or more 3 % slower over 17 sizes
   const int64_t items = BH * sp.n_rt;
-  const int64_t want = std::min<int64_t>(cdiv(Sk, 512), cdiv(2304, items));
+  const int64_t want = std::min<int64_t>(cdiv(Sk, 256), cdiv(768, items));
   sp.chunk = int(cdiv(cdiv(Sk, want), 128) * 128);
-  sp.n_split = items >= 1536 ? 1 : int(cdiv(Sk, sp.chunk));
-  if (sp.n_split == 1) sp.chunk = int(cdiv(Sk, 128) * 128);
-  // columns: row splits where there are few items, of at least 8 tiles of 64 rows
+  sp.n_split = int(cdiv(Sk, sp.chunk));
+  // Columns: row splits up to 768 items, of a 64-row tile or more; up to 2048
+  // where each still has 8 tiles (the first keys are seen by the most rows, so
+  // longer items end unevenly: 16 heads x 16384 rows 1110 us with 2048, 1240 with
+  // 768).  16 heads x 225 rows: 27 us with 8 tiles at least, 17 with one.
   sp.n_kt = int(cdiv(Sk, 64 * tiles));
   const int64_t ci = B * Hkv * sp.n_kt, row_tiles = cdiv(Sq, 64) * sp.group;
-  sp.n_rsplit = int(std::max<int64_t>(1, std::min(cdiv(2048, ci), row_tiles / 8)));
+  sp.n_rsplit = int(std::max<int64_t>(1, std::max(std::min(cdiv(768, ci), row_tiles),
+                                                  std::min(cdiv(2048, ci), row_tiles / 8))));
   if (items * sp.n_split >= (int64_t(1) << 31) || ci * sp.n_rsplit >= (int64_t(1) << 31) ||
       B * Hkv > 65535)
     return MSA_E_HEADS;
