@@ -1278,9 +1278,10 @@ int msa_decode_attention_noalloc(const msa_tensor4* q, const msa_tensor4* k,
 // ---------------------------------------------------------------------------
 namespace {
 
-// Keys of one item's range at most: its buffer descriptors cover below 2 GiB.
+// Keys of one item's range at most: its buffer descriptors cover below 2 GiB (0
+// where two rows do not fit, which an empty cache may say too).
 int64_t rows_max_chunk(const msa_tensor4* k, const msa_tensor4* v) {
-  const int64_t row = std::max({k->stride[2], v->stride[2], k->size[3]}) * 2;
+  const int64_t row = std::clamp(std::max(k->stride[2], v->stride[2]), k->size[3], int64_t(1) << 40) * 2;
   return ((int64_t(1) << 31) - 1024) / row / 128 * 128;
 }
 
@@ -1322,7 +1323,7 @@ int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const
   // own caches: one item per workgroup slot (two a CU), more where a descriptor
   // could not cover an item's keys
   const int64_t triples = B * Hkv * rp.n_rto, units = triples * cdiv(Sc, 128);
-  const int64_t most = rows_max_chunk(k, v) / 128;  // units of an item
+  const int64_t most = std::max<int64_t>(1, rows_max_chunk(k, v) / 128);  // units of an item
   const int64_t n_own = std::min(units, std::max<int64_t>(512, cdiv(units, most)));
   const int64_t row_splits = std::min(n_own, cdiv(Sc, 128));
   if (rp.n_sp + row_splits > kRowsMaxSplit) return MSA_E_SEQ;

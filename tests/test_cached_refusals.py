@@ -145,6 +145,19 @@ def test_prefix_abi_other_head_dim_and_workspace():
     assert lib.msa_shared_prefix_workspace_bytes(REF(ts[0]), REF(big), REF(big), REF(ts[3]), REF(ts[4])) == 0
 
 
+@pytest.mark.parametrize("stride", [1 << 23, 1 << 40, 1 << 62])
+def test_empty_caches_of_any_stride(stride):
+    # rows of an empty cache may lie any distance apart; a division by the
+    # keys of 2 GiB once ended the process here
+    lib = _abi.load_library()
+    ts = [t4(s) for s in (Q, KP, KP)]
+    empty = t4([2, 2, 0, 96], strides=[0, 0, stride, 1])
+    assert lib.msa_shared_prefix_workspace_bytes(*map(REF, ts), REF(empty), REF(empty)) > 0
+    assert lib.msa_decode_accumulate_workspace_bytes(REF(ts[0]), REF(empty), REF(empty)) > 0
+    one = t4([2, 2, 1, 96], strides=[0, 0, stride, 1])
+    assert lib.msa_decode_accumulate_workspace_bytes(REF(ts[0]), REF(one), REF(one)) == 0
+
+
 @pytest.mark.parametrize("kw,want", [
     (dict(q=t4([2, 4, 2, 96]), o=t4([2, 4, 2, 96])), _abi.MSA_E_SEQ),
     (dict(s=t4([2, 2, 49, 1], F32)), _abi.MSA_E_RANK),
