@@ -71,9 +71,10 @@ def _finish(result, call, ts, q: torch.Tensor, out: Optional[torch.Tensor]) -> t
     return result
 
 
-def _check_out(q: torch.Tensor, out: torch.Tensor) -> None:
+def _check_out(q: torch.Tensor, out: torch.Tensor, others=()) -> None:
+    """``out`` may lie where q or a cache does: it is written after they are read."""
     make_out(q, out)
-    check_written("out", out)
+    check_written("out", out, others)
 
 
 @accepts_float32(("q", "k_prefix", "v_prefix", "k_cache", "v_cache"))
@@ -102,7 +103,7 @@ def shared_prefix_attention(
             ``j <= lens[b] - S_q + i``.  Keys behind lens[b] are not used,
             whatever they hold.
         scale: 1/sqrt(D) by default.
-        out: q's shape, q's dtype or fp32.
+        out: q's shape, q's dtype or fp32; may be q itself.
 
     The prefix is read once per 64 query rows (batch x heads of a kv head x
     S_q), not once per sequence.  Equal to dense attention over the
@@ -149,7 +150,7 @@ def decode_accumulate(
             clamped to [0, S]).  Keys behind are not used, whatever they hold,
             and their scores are left as they are.
         scale: 1/sqrt(D) by default.
-        out: q's shape, q's dtype or fp32.
+        out: q's shape, q's dtype or fp32, apart from the scores; may be q itself.
         scores_out: where the sums go; ``scores`` itself by default.
 
     Returns (out, scores_out).  The same call gives the same bits.  With lens[b]
@@ -167,7 +168,7 @@ def decode_accumulate(
                 and scores_out.stride() == scores.stride())
         check_written("scores_out", scores_out, () if same else (("scores", scores),))
     if out is not None:
-        _check_out(q, out)
+        _check_out(q, out, (("scores", scores), ("scores_out", scores_out)))
     s = dense_scale(q.shape[-1]) if scale is None else float(scale)
 
     def call(ts, result):
