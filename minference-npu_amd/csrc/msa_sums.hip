@@ -338,9 +338,7 @@ void sums_cols_kernel(const SumsParams P) {
   constexpr int NKS = Shape::NKS, NT = Shape::TILES;
   constexpr int TK = 16 * NT;  // keys of a wave
   __shared__ __align__(16) unsigned char lds[2 * Shape::STAGE];
-  // m and 1 / l of the tiles' rows: a wave may still weigh a tile's second half
-  // when another stores the tile after next, so three of them
-  __shared__ __align__(16) float stat[3][2][kTileRows];
+  __shared__ __align__(16) float stat[2][2][kTileRows];  // m and 1 / l of the tiles' rows
   const int tid = threadIdx.x, lane = tid & 63, lr = lane >> 4, lc = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   // longest items (first keys) first
@@ -384,9 +382,9 @@ void sums_cols_kernel(const SumsParams P) {
       ++lg;
     }
   };
-  auto store = [&](int stage, int slot) INLINE {
+  auto store = [&](int stage) INLINE {
     part.store(lds + stage * Shape::STAGE + w * Part::BYTES, qr);
-    if (lane < 32) stat[slot][lane >> 4][16 * w + lc] = st;
+    if (lane < 32) stat[stage][lane >> 4][16 * w + lc] = st;
   };
 
   if (t1 > t0) load();  // in flight under the held keys
@@ -438,14 +436,14 @@ void sums_cols_kernel(const SumsParams P) {
 
   if (t1 > t0) {
     __syncthreads();  // the held keys have left LDS
-    store(0, 0);
+    store(0);
     load();
     __syncthreads();
   }
-  int ct = t0 % nt, slot = 0;
+  int ct = t0 % nt;
   for (int t = t0; t < t1; ++t) {
-    const int cs = (t - t0) & 1, next = slot == 2 ? 0 : slot + 1;
-    const float* sp = stat[slot][0];
+    const int cs = (t - t0) & 1;
+    const float* sp = stat[cs][0];
     const int r = rb + kTileRows * ct;
     if (++ct == nt) ct = 0;
     if (active)
@@ -460,10 +458,9 @@ void sums_cols_kernel(const SumsParams P) {
         else
           weigh(rh, false, sp + 32 * half, s);
       }
-    store(1 - cs, next);
+    store(1 - cs);  // the stage that all waves left before the last barrier
     load();
     __syncthreads();
-    slot = next;
     if ((t & 7) == 7) flush();
   }
   flush();
