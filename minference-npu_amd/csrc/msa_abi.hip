@@ -1533,6 +1533,15 @@ int sums_plan(SumsParams& sp, SumsLayout& l, const msa_tensor4* q, const msa_ten
   const int64_t want = std::min<int64_t>(cdiv(Sk, 256), cdiv(768, items));
   sp.chunk = int(cdiv(cdiv(Sk, want), 128) * 128);
   sp.n_split = int(cdiv(Sk, sp.chunk));
+  // One head a kv head and one tile of rows (a window of queries): columns by the
+  // stats pass's items, whose keys' loads run ahead of the work.  32 heads x 64 rows
+  // of 131072 keys of 96 dims: 154 us, 171 by items of 256 keys and all rows.  Keys
+  // beyond the 256 MiB of the last cache do not go there: us streamed / kept, 32
+  // heads, D = 96 and 64: 269 MB 96 / 86, 328 MB 129 / 126, 403 MB 135 / 152, 805 MB
+  // 265 / 295.  Where heads share keys they stay: 8 kv heads x 131072, 32 heads, 301
+  // us streamed, 275 kept.
+  sp.window = Hkv == H && sp.n_rt == 1 && !sp.share;
+  sp.stream = sp.window && BH * Sk * D * 2 > (int64_t(320) << 20);
   // Columns: row splits up to 768 items, of a 64-row tile or more; up to 2048
   // where each still has 8 tiles (the first keys are seen by the most rows, so
   // longer items end unevenly: 16 heads x 16384 rows 1110 us with 2048, 1240 with

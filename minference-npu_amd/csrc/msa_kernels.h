@@ -268,6 +268,7 @@ struct SumsParams {
   float scale_log2;
   int share, stat_rows;       // stats: waves on different rows (1) or keys (0), rows of an item
   int n_rt, n_split, chunk;   // items of a head, key splits, keys of a split
+  int window, stream;         // columns by sums_window_kernel; keys past the caches
   int n_kt, n_rsplit;         // columns: key tiles of an item's four waves, row splits
   float* part;      // n_split > 1: (m, l) [n_split][batch * heads][s_q_pad]
   float* stat_m;    // [batch * heads][s_q_pad]: max of the row's scores, log2 units

@@ -13,11 +13,18 @@
 //     rows of all its heads: S = Q . K^T, lane (lc, lr) gets key lc, rows 4 lr +
 //     i.  Each lane sums its keys' weights in registers.
 // The walked rows go through LDS, 64 a tile, for the four waves of a workgroup
-// (256 rows or keys); with at most 64 rows in all the waves of a stats item
-// take different keys instead.
+// (256 rows or keys); a stats item of fewer rows (see sums_plan) has its waves take
+// different keys, and a window of rows with a kv head a head does its columns the
+// same way (sums_window_kernel).
 // Bound by the exponentials, two for each visible pair (a quarter-rate
-// instruction), with a fused multiply-add and an add beside each.
+// instruction), with a fused multiply-add and an add beside each, and the products,
+// which hardly overlap with them: 16 heads (4 kv) x 16384 rows of 128 dims 1040 us,
+// stats 580 and columns 555, 0.97 PFLOP/s of both score products.  A window is
+// bound by the keys, read twice: 32 heads x 64 rows of 131072 keys of 96 dims 262
+// us, 6.2 TB/s.
 // Sums are fp32 in two levels, in a fixed order.
+
+#include <type_traits>
 
 #include "msa_common.h"
 #include "msa_kernels.h"
@@ -45,6 +52,16 @@ __device__ inline __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, int left, 
                                                    uint32_t stride, int D) {
   const uint32_t n = left > 0 ? uint32_t(min(left, rows) - 1) * stride + 2 * D : 0u;
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), short(0), int(n), 0x00020000);
+}
+
+// A wave's walked keys, not kept in the caches where the call streams them.
+template <typename Part>
+__device__ INLINE inline void load_keys(const SumsParams& P, const Part& part, __amdgpu_buffer_rsrc_t rs,
+                                        u32x4 (&x)[Part::NL]) {
+  if (P.stream)
+    part.template load<2>(rs, 0, x);
+  else
+    part.template load<0>(rs, 0, x);
 }
 
 // Operands of the 16 MT rows from `p` on (`left` exist, the others are 0),
@@ -235,8 +252,8 @@ void sums_stats_kernel(const SumsParams P) {
     unsigned char* mine = lds + w * 2 * Part::BYTES;
     u32x4 kr2[Part::NL];
     auto load = [&](int j0) INLINE {
-      part.load_at(key_rsrc(j0, 16), 0, kr);
-      part.load_at(key_rsrc(j0 + 16, 16), 0, kr2);
+      load_keys(P, part, key_rsrc(j0, 16), kr);
+      load_keys(P, part, key_rsrc(j0 + 16, 16), kr2);
     };
     const int first = j_begin + 32 * w;
     __syncthreads();  // the held rows have left LDS
@@ -483,6 +500,113 @@ void sums_cols_kernel(const SumsParams P) {
   }
 }
 
+// Lane's share of the sums of v[0..7] over its row of 16 lanes: of v[4 b3 + 2 b2 +
+// b1], b the bits of its place in the row.
+__device__ INLINE inline float row_sums(const float (&v)[8], int lc) {
+  const auto from = [](auto ctrl, float x) INLINE {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl(), 0xf, 0xf, true));
+  };
+  const bool b3 = lc & 8, b2 = lc & 4, b1 = lc & 2;
+  float a[4], b[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)  // row_ror:8, lane ^ 8
+    a[i] = (b3 ? v[4 + i] : v[i]) + from(std::integral_constant<int, 0x128>{}, b3 ? v[i] : v[4 + i]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)  // row_half_mirror, lane ^ 7
+    b[i] = (b2 ? a[2 + i] : a[i]) + from(std::integral_constant<int, 0x141>{}, b2 ? a[i] : a[2 + i]);
+  // quad_perm [2,3,0,1], lane ^ 2, then [1,0,3,2], lane ^ 1
+  const float c = (b1 ? b[1] : b[0]) + from(std::integral_constant<int, 0x4e>{}, b1 ? b[0] : b[1]);
+  return c + from(std::integral_constant<int, 0xb1>{}, c);
+}
+
+// Columns of one tile of rows against many keys (one head a kv head, S_q up to the
+// rows a wave holds): the items of the stats pass, the rows held and the keys
+// walked, so that the keys' loads run ahead of the work.
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D > 256 ? 1 : 2)))
+void sums_window_kernel(const SumsParams P) {
+  using Shape = SumsShape<D>;
+  using Part = typename Shape::Part;
+  constexpr int NKS = Shape::NKS;
+  __shared__ __align__(16) unsigned char lds[2 * Shape::STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane >> 4, lc = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bh = blockIdx.x % (P.batch * P.heads), split = blockIdx.x / (P.batch * P.heads);
+  const int b = bh / P.heads, h = bh - b * P.heads;
+  const int shift = P.s_k - P.s_q;
+  const int j_begin = split * P.chunk, j_end = min(j_begin + P.chunk, P.s_k);
+  const float c = P.scale_log2;
+
+  const uint16_t* kbase = reinterpret_cast<const uint16_t*>(P.k) + b * P.k_sb + int64_t(h) * P.k_sh;
+  const uint32_t kss = uint32_t(P.k_ss) * 2u;
+  const Part part(lane, kss);
+  u32x4 kr[2][Part::NL];
+  auto load = [&](int j0) INLINE {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      load_keys(P, part, rows_rsrc(kbase + int64_t(min(j0 + 16 * u, P.s_k - 1)) * P.k_ss,
+                                   P.s_k - j0 - 16 * u, 16, kss, D), kr[u]);
+  };
+  u32x4 qb[MT][NKS];
+  hold_rows<D, MT>(reinterpret_cast<const uint16_t*>(P.q) + b * P.q_sb + int64_t(h) * P.q_sh, P.s_q,
+                   P.q_ss, lane, lds + w * Part::BYTES, qb);
+  float m[MT], inv[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = 16 * mt + lc;
+    m[mt] = r < P.s_q ? P.stat_m[int64_t(bh) * P.s_q_pad + r] : 0.0f;
+    inv[mt] = r < P.s_q ? P.stat_r[int64_t(bh) * P.s_q_pad + r] : 0.0f;
+  }
+  unsigned char* mine = lds + w * 2 * Part::BYTES;
+  float* out = P.sums + b * P.s_sb + h * P.s_sh;
+  const int place = 16 * (lc >> 3) + 4 * lr + 2 * ((lc >> 2) & 1) + ((lc >> 1) & 1);  // row_sums' key
+  const int first = j_begin + 32 * w;
+  __syncthreads();  // the held rows have left LDS
+  load(first);
+  for (int j0 = first; j0 < j_end; j0 += 128) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) part.store(mine + u * Part::BYTES, kr[u]);
+    wave_lds_fence();
+    load(j0 + 128);
+    const int j = j0 + place;
+    const bool stores = (lc & 1) == 0 && j < j_end;
+    const float old = P.add && stores ? out[j] : 0.0f;
+    f32x4 s[MT][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) s[mt][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ks = 0; ks < NKS; ++ks) {
+        const u32x4 a = Part::operand(mine + u * Part::BYTES, 0, lc, lr, ks);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][u] = mfma_qk<T>(a, qb[mt][ks], s[mt][u]);
+      }
+    }
+    float v[8];
+    auto weigh = [&](bool edge) INLINE {
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        v[x] = 0.0f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mt][x >> 2][x & 3], c, -m[mt])), f = inv[mt];
+          if (edge && j0 + 16 * (x >> 2) + 4 * lr + (x & 3) > shift + 16 * mt + lc) e = f = 0.0f;
+          v[x] = __builtin_fmaf(e, f, v[x]);
+        }
+      }
+    };
+    if (j0 + 31 > shift)
+      weigh(true);
+    else
+      weigh(false);
+    wave_lds_fence();
+    const float r = row_sums(v, lc);
+    if (stores) out[j] = P.add ? old + r : r;
+  }
+}
+
 // Column sums of the row splits, in order.
 __global__ __launch_bounds__(256) void sums_reduce_kernel(const SumsParams P) {
   const int j = blockIdx.x * 256 + threadIdx.x;
@@ -512,6 +636,13 @@ hipError_t launch_sums_d(const SumsParams& p, hipStream_t st) {
     hipLaunchKernelGGL(sums_merge_kernel, dim3(uint32_t(bh * p.s_q_pad / 16)), dim3(256), 0, st, p);
     e = hipGetLastError();
     if (e != hipSuccess) return e;
+  }
+  if (p.window) {
+    if (p.stat_rows == 16)
+      hipLaunchKernelGGL((sums_window_kernel<T, D, 1>), ga, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((sums_window_kernel<T, D, NT>), ga, dim3(256), 0, st, p);
+    return hipGetLastError();
   }
   const uint32_t bkv = uint32_t(p.batch) * p.kv_heads;
   hipLaunchKernelGGL((sums_cols_kernel<T, D>), dim3(bkv * p.n_rsplit * p.n_kt), dim3(256), 0, st, p);

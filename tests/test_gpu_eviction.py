@@ -38,6 +38,12 @@ SUMS = [
     (1, 32, 32, 96, 20, 9000, BF16),   # a key tile per wave
     (1, 4, 2, 96, 1500, 1500, BF16),   # row splits
     (1, 4, 4, 128, 16, 20000, FP16),   # key splits
+    (2, 3, 3, 64, 64, 1000, FP16),     # a window, a kv head a head
+    (1, 4, 4, 128, 1, 3001, BF16),
+    (1, 5, 5, 256, 20, 700, BF16),
+    (1, 3, 3, 512, 16, 500, FP16),
+    (2, 2, 2, 96, 50, 50, BF16),
+    (1, 32, 32, 64, 40, 86000, BF16),  # more keys than the caches hold
 ]
 
 
