@@ -44,15 +44,39 @@ __device__ INLINE inline int evict_len(const EvictParams& P, int b) {
 constexpr int kWaves = kSelectThreads / 64;
 constexpr int kBins = kEvictBins;
 
+// x plus its value CTRL lanes away in the row of 16, 0 from outside it.  (A shuffle
+// goes through LDS, whose queue 32 waves of a CU then fill: a third of step 3.)
+template <int CTRL>
+__device__ INLINE inline uint32_t add_from(uint32_t x) {
+  return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over the wave, in every lane.
+__device__ INLINE inline uint32_t wave_sum(uint32_t x) {
+  x = add_from<0x128>(x);  // row_ror:8, 4, 2, 1
+  x = add_from<0x124>(x);
+  x = add_from<0x122>(x);
+  x = add_from<0x121>(x);
+  return (__builtin_amdgcn_readlane(x, 0) + __builtin_amdgcn_readlane(x, 16)) +
+         (__builtin_amdgcn_readlane(x, 32) + __builtin_amdgcn_readlane(x, 48));
+}
+
+// Sum over the wave's lanes up to this one.
+__device__ INLINE inline uint32_t wave_scan(uint32_t x) {
+  const int row = (threadIdx.x >> 4) & 3;
+  x = add_from<0x111>(x);  // row_shr:1, 2, 4, 8
+  x = add_from<0x112>(x);
+  x = add_from<0x114>(x);
+  x = add_from<0x118>(x);
+  const uint32_t a = __builtin_amdgcn_readlane(x, 15), b = a + __builtin_amdgcn_readlane(x, 31),
+                 c = b + __builtin_amdgcn_readlane(x, 47);
+  return x + (row == 0 ? 0u : row == 1 ? a : row == 2 ? b : c);
+}
+
 // Sum over the workgroup's threads before this one.
 __device__ INLINE inline uint32_t scan_before(uint32_t x, uint32_t* wsum) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  uint32_t incl = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint32_t y = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += y;
-  }
+  const uint32_t incl = wave_scan(x);
   if (lane == 63) wsum[w] = incl;
   __syncthreads();
   uint32_t before = 0;
@@ -109,12 +133,6 @@ __device__ INLINE inline int shift_of(int d) { return d == 0 ? 21 : d == 1 ? 10 
 __device__ INLINE inline uint32_t digits_of(int d) { return d == 2 ? 1023u : 2047u; }
 __device__ INLINE inline uint32_t known_of(int d) {
   return d == 0 ? 0u : d == 1 ? 0xffe00000u : 0xfffffc00u;
-}
-
-__device__ INLINE inline uint32_t wave_sum(uint32_t x) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
 }
 
 // The 64-key rows [r0, r1) of a wave (row r: keys 64 r .. 64 r + 63 of the score
@@ -188,30 +206,21 @@ struct Rows {
       weq[w] = n_eq;
     }
     __syncthreads();
-    for (int v = 0; v < w; ++v) {
-      out += wgt[v] + min(weq[v], left - min(left, eq0));
-      eq0 += weq[v];
+#pragma unroll
+    for (int v = 0; v < kWaves - 1; ++v) {
+      const uint32_t g = wgt[v], e = weq[v];
+      out += v < w ? g + min(e, left - min(left, eq0)) : 0u;
+      eq0 += v < w ? e : 0u;
     }
     for (int c0 = r0; c0 < r1; c0 += 64) {
       if (r1 - r0 > 64) masks(c0, T, gt, eq);  // else still there
-      uint32_t ne = __builtin_popcountll(eq), e_before = ne;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t y = __shfl_up(e_before, off, 64);
-        if (lane >= off) e_before += y;
-      }
-      const uint32_t e_total = __shfl(e_before, 63, 64);
+      uint32_t ne = __builtin_popcountll(eq), e_before = wave_scan(ne);
+      const uint32_t e_total = __builtin_amdgcn_readlane(e_before, 63);
       e_before += eq0 - ne;
       const uint32_t take = min(ne, left - min(left, e_before));
       for (; ne > take; --ne) eq &= ~(uint64_t(1) << (63 - __builtin_clzll(eq)));
       const uint64_t m = gt | eq;
-      const uint32_t k = __builtin_popcountll(m);
-      uint32_t k_before = k;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t y = __shfl_up(k_before, off, 64);
-        if (lane >= off) k_before += y;
-      }
+      const uint32_t k = __builtin_popcountll(m), k_before = wave_scan(k);
       const uint32_t at = out + k_before - k;
       for (int i = 0; i < min(64, r1 - c0); ++i) {
         const uint64_t mi = uint64_t(uint32_t(__builtin_amdgcn_readlane(uint32_t(m), i))) |
@@ -220,7 +229,7 @@ struct Rows {
         if ((mi >> lane) & 1)
           pos[ai + __builtin_popcountll(mi & ((uint64_t(1) << lane) - 1))] = 64 * (c0 + i) + lane;
       }
-      out += __shfl(k_before, 63, 64);
+      out += __builtin_amdgcn_readlane(k_before, 63);
       eq0 += e_total;
     }
   }
@@ -262,7 +271,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(const Evic
 
 // grid (stretches, B * kv heads)
 template <int STEP>
-__global__ __launch_bounds__(kSelectThreads) void evict_step_kernel(const EvictParams P) {
+__global__ __launch_bounds__(kSelectThreads) __attribute__((amdgpu_waves_per_eu(8)))
+void evict_step_kernel(const EvictParams P) {
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t wsum[kWaves], wgt[kWaves], weq[kWaves], found[2];
   __shared__ uint32_t s_above[kEvictMaxStretch], s_eq[kEvictMaxStretch];
@@ -280,11 +290,12 @@ __global__ __launch_bounds__(kSelectThreads) void evict_step_kernel(const EvictP
   // of this score row: (T, left) after each digit; keys above it of each stretch
   uint32_t* state = P.state + int64_t(blockIdx.y) * (6 + 3 * kEvictMaxStretch);
   uint32_t* above = state + 6;
-  uint32_t T = 0, left = row.want;
+  uint32_t T = 0, left = row.want, above_before = 0;
   if (STEP > 1 && row.want > 0) {
     T = state[2 * (STEP - 2)];
     left = state[2 * (STEP - 2) + 1];
   }
+  if (STEP == 3 && row.want > 0 && tid < x) above_before = above[tid] + above[kEvictMaxStretch + tid];
   const uint32_t* last = nullptr;  // the row's histograms of the digit before
   if (STEP > 0 && row.want > 0) {
     last = P.hist + (int64_t(STEP - 1) * gridDim.y + blockIdx.y) * P.n_stretch * kBins;
@@ -318,7 +329,7 @@ __global__ __launch_bounds__(kSelectThreads) void evict_step_kernel(const EvictP
       state[2 * (STEP - 1) + 1] = left;
     }
   }
-  // this stretch's rows of 64 keys
+  // this stretch's rows of 64 keys, their loads under those of the histograms
   const int rows = (row.n + 63) / 64, s0 = min(rows, x * (P.stretch / 64));
   const int s1 = min(rows, s0 + P.stretch / 64), per = (s1 - s0 + kWaves - 1) / kWaves;
   Rows<8> mine(row, min(s1, s0 + w * per), min(s1, s0 + w * per + per));
@@ -336,12 +347,14 @@ __global__ __launch_bounds__(kSelectThreads) void evict_step_kernel(const EvictP
     if (row.want > 0) {
       if (tid < x) {
         s_eq[tid] = last[tid * kBins + (T & 1023u)];
-        s_above[tid] += above[tid] + above[kEvictMaxStretch + tid];
+        s_above[tid] += above_before;
       }
       __syncthreads();
-      for (int y = 0; y < x; ++y) {
-        out += s_above[y] + min(s_eq[y], left - min(left, eq0));
-        eq0 += s_eq[y];
+#pragma unroll
+      for (int y = 0; y < kEvictMaxStretch - 1; ++y) {
+        const uint32_t a = s_above[y], e = s_eq[y];
+        out += y < x ? a + min(e, left - min(left, eq0)) : 0u;
+        eq0 += y < x ? e : 0u;
       }
     } else {
       T = 0xffffffffu;
