@@ -44,8 +44,9 @@ __device__ INLINE inline int evict_len(const EvictParams& P, int b) {
 constexpr int kWaves = kSelectThreads / 64;
 constexpr int kBins = kEvictBins;
 
-// x plus its value CTRL lanes away in the row of 16, 0 from outside it.  (A shuffle
-// goes through LDS, whose queue 32 waves of a CU then fill: a third of step 3.)
+// x plus its value CTRL lanes away in the row of 16, 0 from outside it.  (Shuffles
+// go through LDS, which 32 waves of a CU then wait for: with them the four steps of
+// 64 rows x 65536 scores take 62 us instead of 54.)
 template <int CTRL>
 __device__ INLINE inline uint32_t add_from(uint32_t x) {
   return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf, true));
@@ -329,7 +330,7 @@ void evict_step_kernel(const EvictParams P) {
       state[2 * (STEP - 1) + 1] = left;
     }
   }
-  // this stretch's rows of 64 keys, their loads under those of the histograms
+  // this stretch's rows of 64 keys
   const int rows = (row.n + 63) / 64, s0 = min(rows, x * (P.stretch / 64));
   const int s1 = min(rows, s0 + P.stretch / 64), per = (s1 - s0 + kWaves - 1) / kWaves;
   Rows<8> mine(row, min(s1, s0 + w * per), min(s1, s0 + w * per + per));
