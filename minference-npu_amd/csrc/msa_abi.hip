@@ -1315,7 +1315,7 @@ int rows_plan(RowsParams& rp, const msa_tensor4* q, const msa_tensor4* kp, const
   rp.s_q = int(Sq);
   rp.s_p = int(Sp);
   rp.s_c = int(Sc);
-  rows_forms(rp, R, rows, int(D));
+  rows_forms(rp, R, rows, int(D), kp == nullptr);
   rp.n_rt = int(cdiv(R, rp.prefix_rows));
   rp.n_rto = int(cdiv(rows, rp.own_rows));
   rows_split(Sp, std::min<int64_t>(cdiv(Sp, 256), cdiv(512, rp.n_rt * Hkv)),

@@ -15,6 +15,9 @@
 // In both a wave has 64 contiguous keys at a time: ballots give the kept ones,
 // lane i keeps the masks of the wave's i-th 64 keys, and one exchange between
 // the waves gives the places.
+//   Bound by latency, of the histograms' way from launch to launch and the scans:
+//   8 x 8 heads x 65536 scores (17 MB) 8 + 13 + 12 + 22 us; select, 32 rows of 4113,
+//   14 us.
 // gather: the kept rows of K and V and their scores.  Bound by memory, each kept
 //   row read and written once: 8 x 8 heads, 16384 of 65536 keys of 128 dims take
 //   190 us for 1.07 GB (5.6 TB/s).

@@ -368,8 +368,9 @@ hipError_t launch_attention_vs(const AttnParams& p, int dtype, int out_dtype, in
 hipError_t launch_vs_build(const VsBuildParams& p, int n_bs, hipStream_t st);
 hipError_t launch_vs_estimate(const VsEstParams& p, int dtype, int D, hipStream_t st);
 hipError_t launch_block_lists(const ListParams& p, hipStream_t st);
-// Item forms of `rows` prefix rows a kv head and `seq_rows` rows of a sequence.
-void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D);
+// Item forms of `rows` prefix rows a kv head and `seq_rows` rows of a sequence;
+// scores: of a call that leaves raw scores.
+void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D, bool scores);
 hipError_t launch_rows(const RowsParams& p, bool accumulate, int dtype, int out_dtype, int D,
                        hipStream_t st);
 int sums_tiles(int D);  // 16-row (16-key) tiles of a stats (columns) item

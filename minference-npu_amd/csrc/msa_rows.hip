@@ -11,26 +11,32 @@
 // keys; the raw scores go to the workspace and the second launch adds the
 // normalised weights, summed over the heads of a kv head, to a score per key.
 //
-// A workgroup takes one item: up to 16 MT rows of one kv head against one key
-// range (of the prefix, or of one sequence's own cache), wave w its 32-key
-// blocks w, w + 4, ...
+// A workgroup takes one item: rows of one kv head against one key range (of the
+// prefix, or of one sequence's own cache).
 //   S^T = K . Q^T on the 16-bit 16x16x32 MFMA (exact products, fp32 sums): A
 //     = 16 keys from their rows, B = 16 query rows, held for the whole item.
 //     Lane (lc, lr) gets query lc, keys 4 lr + i of the 16.
 //   O^T += V^T . P^T on the same MFMA, 32 keys a step.  The order of the 32 is
 //     free as long as V and P share it: slot 8 lr + j is key 4 lr + j of the
 //     block's first 16 for j < 4, of the second 16 after that, which is where
-//     P already lies.  V (A operand) is loaded by rows, a lane holding E = D /
-//     16 (8 from D = 128 on) dims of its 8 keys, and pairs of keys are put
-//     together by byte permutes; MFMA e takes dim E lc + e of every lane.
-// K goes through LDS (each wave its own block, no barrier), V straight from its
-// rows; both are read once per item.  Softmax statistics
-// and O are fp32; a row's running max moves only when a block exceeds it by
-// 2^kSlack.  P is rounded to the inputs' type twice, P and what that rounding
-// left, so the product's error stays below the output's own rounding (kTwoParts
-// names the exception).
-// Each item leaves O and (m, l) of its rows in the workspace; the combine
-// kernel merges the items of a row.
+//     P already lies.
+// kOwn (up to 16 rows): wave w takes the 32-key blocks w, w + 4, ...; K goes
+//   through LDS (each wave its own block, no barrier), V straight from its rows, a
+//   lane holding E = D / 16 (8 from D = 128 on) dims of its 8 keys, and pairs of
+//   keys are put together by byte permutes; MFMA e takes dim E lc + e of every lane.
+//   Bound by memory: 16 rows on 8 x 1 M keys of 128 dims 6.7 TB/s; decode of 8 ragged
+//   sequences on 8 x 65536 x 128 265 us, 5.5 TB/s, the raw scores' stores 20 of it.
+// kTile (up to 64 MT rows): the waves share 64 keys in LDS and take 16 MT rows each.
+//   Bound by the sum of the products (two of P where kTwoParts says so) and the
+//   softmax, which hardly overlap: 128 rows a kv head on 8 x 65536 x 128, with 32 x
+//   8 own caches of up to 1024 keys, 84 us (4.3 TB/s); 512 rows on 8 x 32768 x 128
+//   fp16, with 128 x 8 caches of up to 512, 129 us (0.55 PFLOP/s).
+// Softmax statistics and O are fp32; a row's running max moves only when a block
+// exceeds it by 2^kSlack.  P is rounded to the inputs' type twice, P and what that
+// rounding left, so the product's error stays below the output's own rounding
+// (kTwoParts names the exception).
+// Each item leaves O and (m, l) of its rows in the workspace; the second launch
+// merges the items of a row (4 us for 128 rows, 10 for 1024, 13 for 4096).
 
 #include "msa_common.h"
 #include "msa_kernels.h"
@@ -163,8 +169,8 @@ __device__ INLINE inline void add_nonfinite(const Item& it, int j0, int lane,
   }
 }
 
-// Forms of an item: kOwn + MT: up to 16 MT rows, the four waves take different
-// keys; kTile + MT: up to 64 MT rows, 16 MT a wave, the waves share the keys.
+// Forms of an item (rows_forms): kOwn + MT: up to 16 MT rows, the four waves take
+// different keys; kTile + MT: up to 64 MT rows, 16 MT a wave, the waves share the keys.
 constexpr int kOwn = 0, kTile = 8;
 constexpr int form_rows(int form) {
   return form >= kTile ? 64 * (form - kTile) : 16 * form;
@@ -991,11 +997,11 @@ void launch_prefix_k(const RowsParams& p, hipStream_t st) {
 template <typename T, int D, bool CAUSAL>
 void launch_prefix_f(const RowsParams& p, hipStream_t st) {
   if constexpr (D <= 128) {
-    if constexpr (CAUSAL)
-      if (p.own_form == kTile + 2) return launch_prefix_k<T, D, kTile + 2, kTile + 2, true>(p, st);
+    if (p.own_form == kTile + 2)
+      return p.prefix_form == kTile + 2 ? launch_prefix_k<T, D, kTile + 2, kTile + 2, CAUSAL>(p, st)
+                                        : launch_prefix_k<T, D, kTile + 1, kTile + 2, CAUSAL>(p, st);
     if (p.prefix_form == kTile + 2) return launch_prefix_k<T, D, kTile + 2, kOwn + 1, CAUSAL>(p, st);
     if (p.prefix_form == kTile + 1) return launch_prefix_k<T, D, kTile + 1, kOwn + 1, CAUSAL>(p, st);
-    if (p.prefix_form == kOwn + 2) return launch_prefix_k<T, D, kOwn + 2, kOwn + 1, CAUSAL>(p, st);
   }
   launch_prefix_k<T, D, kOwn + 1, kOwn + 1, CAUSAL>(p, st);
 }
@@ -1043,14 +1049,21 @@ hipError_t launch_rows_t(const RowsParams& p, bool accumulate, int D, hipStream_
 
 }  // namespace
 
-void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D) {
-  const bool tiles = D <= 128;
-  p.own_form = tiles && p.s_q > 1 && seq_rows > 32 ? kTile + 2 : kOwn + 1;
-  p.prefix_form = !tiles || rows <= 16       ? kOwn + 1
-                  : p.own_form > kTile       ? kTile + 2
-                  : rows <= 32               ? kOwn + 2
-                  : rows <= 64               ? kTile + 1
-                                             : kTile + 2;
+// us of a call, bf16, by form.
+// Prefix 8 x 65536 x 128:   16 rows   24   32   48   64   96
+//   kOwn + 1                54   61   61  106   96  182
+//   kTile + 1               53   54   54   55   57   77
+//   kTile + 2               55   55   55   58   60   65
+// and 32 x 4096 x 96 with 4 rows: kOwn + 1 18.5, kTile + 1 19.1 (most waves of a
+// kTile item of few rows only load).
+// Own caches 8 x 8 x 4096 x 128 with 8 / 16 / 20 / 32 rows: kOwn + 1 36 / 40 / 59 /
+// 62, kTile + 2 34 / 36 / 36 / 38; with 16 rows, 4 x 32 x 200 x 96 behind 1000 shared
+// keys, 17 / 20.
+// Above 128 dims O of a kTile item does not fit the registers; raw scores are kOwn's.
+void rows_forms(RowsParams& p, int64_t rows, int64_t seq_rows, int D, bool scores) {
+  const bool tiles = D <= 128 && !scores;
+  p.own_form = tiles && seq_rows > 16 ? kTile + 2 : kOwn + 1;
+  p.prefix_form = !tiles || rows <= 16 ? kOwn + 1 : rows <= 64 ? kTile + 1 : kTile + 2;
   p.prefix_rows = form_rows(p.prefix_form);
   p.own_rows = int(seq_rows < form_rows(p.own_form) ? seq_rows : form_rows(p.own_form));
 }

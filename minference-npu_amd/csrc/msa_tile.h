@@ -2,9 +2,9 @@
 //
 // An MFMA operand wants 16 rows in 16 neighbouring lanes, 16 bytes of each: read
 // like that from global memory every lane of a pass touches another cache line,
-// which the L1 serves slowly at most row strides (the stats pass of 16 heads x
-// 16384 x 128 read in place: 1000 us; through LDS and shared by four waves: see
-// msa_sums.hip).  Here a wave loads whole rows, neighbouring lanes on
+// which the L1 serves slowly at most row strides (the weight sums' stats pass of 16
+// heads x 16384 x 128 read in place: 1000 us; through LDS, shared by four waves:
+// 580).  Here a wave loads whole rows, neighbouring lanes on
 // neighbouring 16 bytes, into registers, later writes them to LDS, and reads
 // operands back.  The 16-byte chunks of a row are permuted by its number so that
 // neither side has bank conflicts: 16 lanes that read one chunk of 16 rows hit

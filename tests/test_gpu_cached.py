@@ -67,6 +67,11 @@ PREFIX = [
     (1, 8, 8, 96, 20000, 600, 1, BF16, None),
     (130, 2, 1, 64, 40, 260, 1, BF16, [(7 * i) % 261 for i in range(130)]),
     (2, 2, 2, 128, 9000, 300, 40, BF16, [300, 150]),
+    (3, 6, 2, 128, 200, 90, 6, FP16, [90, 5, 40]),      # 18 rows of a sequence, 54 in all
+    (2, 32, 1, 96, 300, 150, 1, BF16, [150, 70]),       # 32 heads of a kv head
+    (1, 20, 1, 64, 100, 300, 1, FP16, None),
+    (9, 32, 1, 128, 500, 70, 1, BF16, [70 - 8 * i for i in range(9)]),
+    (2, 8, 4, 96, 257, 60, 9, BF16, [60, 9]),
 ]
 
 
