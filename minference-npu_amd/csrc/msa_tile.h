@@ -23,14 +23,13 @@ struct Tile {
   static_assert(ROWS * NCH % 64 == 0, "a tile is whole wave loads");
 
   // Place of chunk c of row r.  8 chunks: two rows fill the banks, so pairs of
-  // rows take turns; 12: rows start 12 bank groups apart, groups of four rows
-  // shift by one; 16 and more: every row its own permutation.
+  // rows take turns; 12: rows start 12 bank groups apart, so four rows take every
+  // fourth group and groups of four rows take turns among them; 16 and more: every
+  // row its own permutation.
   __device__ static int place(int r, int c) {
     if constexpr (NCH == 8) return r * 8 + (c ^ ((r >> 1) & 7));
-    else if constexpr (NCH == 12) {
-      const int x = c + ((r >> 2) & 3);
-      return r * 12 + (x >= 12 ? x - 12 : x);
-    } else return r * NCH + (c ^ (r & 15));
+    else if constexpr (NCH == 12) return r * 12 + (c ^ ((r >> 2) & 3));
+    else return r * NCH + (c ^ (r & 15));
   }
 
   uint32_t off[NL];    // byte offset of this lane's i-th chunk from the tile's first row
