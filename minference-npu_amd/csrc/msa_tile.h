@@ -24,12 +24,15 @@ struct Tile {
 
   // Place of chunk c of row r.  8 chunks: two rows fill the banks, so pairs of
   // rows take turns; 12: rows start 12 bank groups apart, so four rows take every
-  // fourth group and groups of four rows take turns among them; 16 and more: every
-  // row its own permutation.
+  // fourth group and groups of four rows take turns among them, such that groups
+  // 0 and 3 of one chunk and 1 and 2 of the next do not meet either (an operand read
+  // takes its lanes in this order); 16 and more: every row its own permutation.
   __device__ static int place(int r, int c) {
     if constexpr (NCH == 8) return r * 8 + (c ^ ((r >> 1) & 7));
-    else if constexpr (NCH == 12) return r * 12 + (c ^ ((r >> 2) & 3));
-    else return r * NCH + (c ^ (r & 15));
+    else if constexpr (NCH == 12) {
+      const int g = (r >> 2) & 3;
+      return r * 12 + (c & ~3) + ((((c & 1) << 1) | ((c >> 1) & 1)) ^ g ^ (g >> 1));
+    } else return r * NCH + (c ^ (r & 15));
   }
 
   uint32_t off[NL];    // byte offset of this lane's i-th chunk from the tile's first row
