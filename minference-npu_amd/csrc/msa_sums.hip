@@ -18,10 +18,10 @@
 // same way (sums_window_kernel).
 // Bound by the exponentials, two for each visible pair (a quarter-rate
 // instruction), with a fused multiply-add and an add beside each, and the products,
-// which hardly overlap with them: 16 heads (4 kv) x 16384 rows of 128 dims 1040 us,
-// stats 580 and columns 555, 0.97 PFLOP/s of both score products.  A window is
-// bound by the keys, read twice: 32 heads x 64 rows of 131072 keys of 96 dims 262
-// us, 6.2 TB/s.
+// which hardly overlap with them: 16 heads (4 kv) x 16384 rows of 128 dims 1024 us,
+// stats 574 and columns 551 by themselves, 1.07 PFLOP/s of both score products.  A
+// window is bound by the keys, read twice: 32 heads x 64 rows of 131072 keys of 96
+// dims 119 + 138 us, 6.3 TB/s.
 // Sums are fp32 in two levels, in a fixed order.
 
 #include <type_traits>
