@@ -16,8 +16,8 @@
 // lane i keeps the masks of the wave's i-th 64 keys, and one exchange between
 // the waves gives the places.
 //   Bound by latency, of the histograms' way from launch to launch and the scans:
-//   8 x 8 heads x 65536 scores (17 MB) 8 + 13 + 12 + 22 us; select, 32 rows of 4113,
-//   14 us.
+//   8 x 8 heads x 65536 scores (17 MB) 8 + 13 + 12 + 20 us; select, 32 rows of 4113,
+//   12 us.
 // gather: the kept rows of K and V and their scores.  Bound by memory, each kept
 //   row read and written once: 8 x 8 heads, 16384 of 65536 keys of 128 dims take
 //   190 us for 1.07 GB (5.6 TB/s).
@@ -49,7 +49,7 @@ constexpr int kBins = kEvictBins;
 
 // x plus its value CTRL lanes away in the row of 16, 0 from outside it.  (Shuffles
 // go through LDS, which 32 waves of a CU then wait for: with them the four steps of
-// 64 rows x 65536 scores take 62 us instead of 54.)
+// 64 rows x 65536 scores take 8 us more.)
 template <int CTRL>
 __device__ INLINE inline uint32_t add_from(uint32_t x) {
   return x + uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xf, 0xf, true));
@@ -175,7 +175,7 @@ struct Rows {
   // of those equal to T, lane i for row c0 + i; at most 64 rows.
   __device__ INLINE void masks(int c0, uint32_t T, uint64_t& gt, uint64_t& eq) {
     gt = eq = 0;
-#pragma unroll
+#pragma unroll 1  // most waves take one turn, and fetching the code of eight cost 3 us
     for (int q = 0; q < 64 / R; ++q) {
       if (c0 + q * R >= r1) break;
       if (r1 - r0 > R) load(c0 + q * R);
@@ -320,11 +320,20 @@ void evict_step_kernel(const EvictParams P) {
     // keys above the digit: of every stretch before the last step, of this one
     // otherwise
     const bool t_above = kBins - 1 - 2 * tid > digit, n_above = kBins - 2 - 2 * tid > digit;
-#pragma unroll
-    for (int y = 0; y < kEvictMaxStretch; ++y) {
-      if (STEP < 3 ? y != x : y >= P.n_stretch) continue;
-      const uint32_t sum = wave_sum((t_above ? part[y].y : 0u) + (n_above ? part[y].x : 0u));
+    const auto add_above = [&](int y, uint2 p) INLINE {
+      const uint32_t sum = wave_sum((t_above ? p.y : 0u) + (n_above ? p.x : 0u));
       if ((tid & 63) == 0 && sum) atomicAdd(&s_above[y], sum);
+    };
+    if constexpr (STEP == 3) {
+#pragma unroll
+      for (int y = 0; y < kEvictMaxStretch; ++y)
+        if (y < P.n_stretch) add_above(y, part[y]);
+    } else {
+      uint2 p = part[0];
+#pragma unroll
+      for (int y = 1; y < kEvictMaxStretch; ++y)
+        if (y == x) p = part[y];
+      add_above(x, p);
     }
     __syncthreads();
     if (STEP < 3 && tid == 0) above[(STEP - 1) * kEvictMaxStretch + x] = s_above[x];
