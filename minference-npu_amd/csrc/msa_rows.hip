@@ -977,16 +977,19 @@ __global__ __launch_bounds__(256) void rows_weights_kernel(const RowsParams P, i
   const float* raw = P.raw + (int64_t(b) * P.heads + kvh * P.group) * P.raw_row;
   const float* in = P.w_in + b * P.wi_sb + kvh * P.wi_sh;
   float* out = P.w_out + b * P.wo_sb + kvh * P.wo_sh;
+  const int j = j0 + 4 * tid;  // rows of raw are whole 16 bytes
+  if (j >= len) return;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int g = 0; g < P.group; ++g) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(raw + g * P.raw_row + j);
 #pragma unroll
-  for (int q = 0; q < kWeightKeys / 256; ++q) {
-    const int j = j0 + 256 * q + tid;
-    if (j >= len) break;
-    float acc = 0.0f;
-    for (int g = 0; g < P.group; ++g)
-      acc += sR[g] * __builtin_amdgcn_exp2f(
-                         __builtin_fmaf(raw[g * P.raw_row + j], P.scale_log2, -sM[g]));
-    out[j] = in[j] + acc;
+    for (int i = 0; i < 4; ++i)
+      acc[i] += sR[g] * __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], P.scale_log2, -sM[g]));
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (j + i < len) out[j + i] = in[j + i] + acc[i];
 }
 
 template <typename T, int D, int PF, int OF, bool CAUSAL>
